@@ -1,0 +1,328 @@
+// Keys and values of a cache entry in eight bits (csrc/cache_quant.cuh): append, read-back, and attention for the sizes and types
+// that csrc/attention_quant.cu does not take.
+//
+// The reference's cache holds half precision only (src/qwen_kernels.cu:111-126 writes it).
+#include "cache_quant.cuh"
+
+using namespace cq;
+
+// ---- append ------------------------------------------------------------------------------------------------------------------
+// Rows of `qkv` are [Hq heads | Hkv key heads | Hkv value heads | ...] of D numbers, `row_stride` apart.  A query or key head x
+// becomes x / sqrt(mean(x^2) + eps) * w (eps > 0; w: D numbers or null), then its first 2 rot_half numbers are turned by the
+// row's angles as pairs (t, t + rot_half); queries are rounded to q_out, keys and values quantised from float32 - one rounding - into
+// the page of the row's position.  The scale needs the whole row's largest magnitude before the first code is written.
+struct AppendParams {
+    const void* qkv;
+    int row_stride;
+    const float* bias;         // per column of [q | k | v], or null
+    const float* q_norm;
+    const float* k_norm;
+    float eps;                 // 0: no norm
+    const float* cos_t;        // [table_len, rot_half]
+    const float* sin_t;
+    int rot_half, table_len;
+    const int* positions;
+    const int* row_segment;
+    const int* block_table;
+    int table_stride;
+    uint8_t* k_codes;          // [num_pages, Hkv, page_size, D]
+    uint8_t* v_codes;
+    uint8_t* k_scales;         // [num_pages, Hkv, page_size]
+    uint8_t* v_scales;
+    int num_pages;
+    void* q_out;               // [T, Hq * D]
+    int T, Hq, Hkv, D, page_size, write_kv;
+    int* err;
+};
+
+// Where the row's keys lie: index of its slot of head 0 among the pool's rows; -1: no page.
+__device__ __forceinline__ long long slot_of(const AppendParams& p, int row, int pos, bool report) {
+    const int place = pos / p.page_size;
+    const int page = pos >= 0 && place < p.table_stride ? p.block_table[(size_t)p.row_segment[row] * p.table_stride + place] : -1;
+    if (page < 0 || page >= p.num_pages) {
+        if (report) atomicOr(p.err, KVB_DEV_BAD_PAGE);
+        return -1;
+    }
+    return (long long)page * p.Hkv * p.page_size + pos % p.page_size;
+}
+
+// Any head size, float32 or bfloat16: a warp a (row, head).  A number is made twice, for the largest and for its code.
+template <typename T, int STORE>
+__global__ void append_quant_any_kernel(const AppendParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), lane = threadIdx.x & 31;
+    const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (item >= (long long)p.T * heads) return;
+    const int row = (int)(item / heads), head = (int)(item - (long long)row * heads), D = p.D;
+    const int pos = p.positions[row];
+    const bool is_q = head < p.Hq, is_v = head >= p.Hq + p.Hkv;
+    const T* x = (const T*)p.qkv + (size_t)row * p.row_stride + (size_t)head * D;
+    const float* bias = p.bias ? p.bias + (size_t)head * D : nullptr;
+    const float* weight = is_q ? p.q_norm : p.k_norm;
+    auto biased = [&](int d) { return to_f32<T>(x[d]) + (bias ? bias[d] : 0.f); };
+    float inv = 1.f;
+    if (!is_v && p.eps > 0.f) {
+        float sum = 0.f;
+        for (int d = lane; d < D; d += 32) { const float v = biased(d); sum = fmaf(v, v, sum); }
+        inv = rsqrtf(warp_sum(sum) / D + p.eps);
+    }
+    const bool normed = !is_v && p.eps > 0.f;
+    auto scaled = [&](int d) { const float v = biased(d); return normed ? (weight ? v * inv * weight[d] : v * inv) : v; };
+    const bool pos_ok = p.rot_half == 0 || (pos >= 0 && pos < p.table_len);
+    if (!pos_ok && lane == 0) atomicOr(p.err, KVB_DEV_BAD_POS);
+    const float* cr = p.cos_t + (size_t)(pos_ok ? pos : 0) * p.rot_half;
+    const float* sr = p.sin_t + (size_t)(pos_ok ? pos : 0) * p.rot_half;
+    auto value = [&](int d) {
+        const float v = scaled(d);
+        if (is_v || d >= 2 * p.rot_half) return v;
+        const bool low = d < p.rot_half;
+        const int t = low ? d : d - p.rot_half;
+        const float partner = scaled(low ? d + p.rot_half : t);
+        return low ? v * cr[t] - partner * sr[t] : v * cr[t] + partner * sr[t];
+    };
+    if (is_q) {
+        T* out = (T*)p.q_out + ((size_t)row * p.Hq + head) * D;
+        for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(value(d));
+        return;
+    }
+    const long long slot = slot_of(p, row, pos, lane == 0);
+    if (slot < 0) return;
+    uint32_t top = 0u;
+    for (int d = lane; d < D; d += 32) top = max(top, __float_as_uint(value(d)) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const int byte = scale_byte<STORE>(top);
+    const float down = scale_down(byte);
+    const long long at = slot + (long long)(is_v ? head - p.Hq - p.Hkv : head - p.Hq) * p.page_size;
+    uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + at * D;
+    for (int d = lane; d < D; d += 32) codes[d] = (uint8_t)code_of<STORE>(value(d), down);
+    if (lane == 0) (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)byte;
+}
+
+template <typename T>
+static int append_any(const AppendParams& p, int store, cudaStream_t stream) {
+    const long long items = (long long)p.T * (p.Hq + (p.write_kv ? 2 * p.Hkv : 0));
+    const dim3 grid((unsigned)((items + 7) / 8));
+    if (store == KVB_E4M3) kvb_launch(append_quant_any_kernel<T, KVB_E4M3>, grid, dim3(256), 0, stream, p);
+    else kvb_launch(append_quant_any_kernel<T, KVB_INT8>, grid, dim3(256), 0, stream, p);
+    return kvb_launch_status();
+}
+
+KVB_API int kvb_append_quant(int dtype, int store, const void* qkv, int row_stride, const float* bias, const float* q_norm, const float* k_norm,
+                             float eps, const float* cos_t, const float* sin_t, int rot_half, int table_len, const int* positions,
+                             const int* row_segment, const int* block_table, int table_stride, void* k_codes, void* v_codes, void* k_scales,
+                             void* v_scales, int num_pages, void* q_out, int T, int Hq, int Hkv, int D, int page_size, int write_kv, int* err,
+                             cudaStream_t stream) {
+    if (T <= 0) return KVB_OK;
+    if (store != KVB_E4M3 && store != KVB_INT8) return KVB_ERR_DTYPE;
+    if (D < 1 || Hq < 0 || Hkv < 1 || page_size < 1 || rot_half < 0 || 2 * rot_half > D || num_pages < 1) return KVB_ERR_SHAPE;
+    if (row_stride < (Hq + (write_kv ? 2 * Hkv : 0)) * D || (rot_half > 0 && (!cos_t || !sin_t))) return KVB_ERR_SHAPE;
+    if ((long long)T * (Hq + 2 * Hkv) > 0x7fffffffll) return KVB_ERR_LIMIT;
+    if (Hq + (write_kv ? 2 * Hkv : 0) == 0) return KVB_OK;
+    const AppendParams p = {qkv, row_stride, bias, q_norm, k_norm, eps, cos_t, sin_t, rot_half, table_len, positions, row_segment, block_table,
+                            table_stride, (uint8_t*)k_codes, (uint8_t*)v_codes, (uint8_t*)k_scales, (uint8_t*)v_scales, num_pages, q_out, T, Hq, Hkv, D,
+                            page_size, write_kv, err};
+    if (dtype == KVB_BF16) return append_any<bf16>(p, store, stream);
+    if (dtype == KVB_F32) return append_any<float>(p, store, stream);
+    return KVB_ERR_DTYPE;
+}
+
+// ---- read-back ---------------------------------------------------------------------------------------------------------------
+// Blocks of 64 keys of every segment, one segment after the other.  ranges: int32 [S + 1, 3] - the blocks before the segment's, and
+// its blocks: 0 .. kept - 1, then from `first` on (kernels/cache_plan.py).  Block i becomes page i of k_out / v_out [n, Hkv, 64, D], and
+// out_table[segment, block] = i.  Keys that no row of the segment sees (behind its end; before the first row's window, unless among the
+// first `keep`) become zeros, whatever their pages hold.
+constexpr int READ_BLOCK = 64;
+struct ExpandParams {
+    const uint8_t* k_codes;
+    const uint8_t* v_codes;
+    const uint8_t* k_scales;
+    const uint8_t* v_scales;
+    int num_pages;
+    const int* block_table;
+    int table_stride, page_size;
+    const int* ranges;
+    int segments;
+    const int* seg_q_len;
+    const int* seg_kv_len;
+    int reach, keep;
+    void* k_out;
+    void* v_out;
+    int* out_table;
+    int out_stride, Hkv, D;
+    int* err;
+};
+
+// The segment that block i belongs to, and which of its blocks it is.
+__device__ __forceinline__ void find_block(const ExpandParams& p, int i, int& seg, int& block) {
+    int lo = 0;
+    for (int hi = p.segments; hi - lo > 1;) { const int mid = (lo + hi) >> 1; if (p.ranges[3 * mid] <= i) lo = mid; else hi = mid; }
+    const int j = i - p.ranges[3 * lo], kept = p.ranges[3 * lo + 1];
+    seg = lo;
+    block = j < kept ? j : p.ranges[3 * lo + 2] + j - kept;
+}
+
+template <typename T, int STORE>
+__global__ void expand_any_kernel(const ExpandParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int i = blockIdx.x, hk = blockIdx.y, D = p.D;
+    const bool values = blockIdx.z == 1;
+    int seg, block;
+    find_block(p, i, seg, block);
+    const int kv_len = p.seg_kv_len[seg], lo = first_seen_key(kv_len - p.seg_q_len[seg], p.reach), keep = p.reach > 0 ? p.keep : 0;
+    if (hk == 0 && !values && threadIdx.x == 0 && block < p.out_stride) p.out_table[(size_t)seg * p.out_stride + block] = i;
+    const uint8_t* codes = values ? p.v_codes : p.k_codes;
+    const uint8_t* scales = values ? p.v_scales : p.k_scales;
+    T* out = (T*)(values ? p.v_out : p.k_out) + ((size_t)i * p.Hkv + hk) * READ_BLOCK * D;
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < READ_BLOCK; r += blockDim.x >> 5) {
+        const int key = block * READ_BLOCK + r;
+        long long at = -1;
+        if (key < kv_len && (key >= lo || key < keep)) {
+            const int place = key / p.page_size;
+            const int page = place < p.table_stride ? p.block_table[(size_t)seg * p.table_stride + place] : -1;
+            if (page >= 0 && page < p.num_pages) at = ((long long)page * p.Hkv + hk) * p.page_size + key % p.page_size;
+            else if (lane == 0) atomicOr(p.err, KVB_DEV_BAD_PAGE);
+        }
+        const float up = at >= 0 ? scale_up(scales[at]) : 0.f;
+        for (int d = lane; d < D; d += 32)
+            out[(size_t)r * D + d] = from_f32<T>(at >= 0 ? code_value<STORE>(codes[at * D + d]) * up : 0.f);
+    }
+}
+
+KVB_API int kvb_cache_expand(int dtype, int store, const void* k_codes, const void* v_codes, const void* k_scales, const void* v_scales, int num_pages,
+                             const int* block_table, int table_stride, int page_size, const int* ranges, int segments, int n,
+                             const int* seg_q_len, const int* seg_kv_len, int reach, int keep, void* k_out, void* v_out, int* out_table, int out_stride, int Hkv, int D,
+                             int* err, cudaStream_t stream) {
+    if (n <= 0) return KVB_OK;
+    if (store != KVB_E4M3 && store != KVB_INT8) return KVB_ERR_DTYPE;
+    if (D < 1 || Hkv < 1 || Hkv > 65535 || page_size < 1 || num_pages < 1 || keep < 0 || segments < 1) return KVB_ERR_SHAPE;
+    const ExpandParams p = {(const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scales, (const uint8_t*)v_scales, num_pages, block_table,
+                            table_stride, page_size, ranges, segments, seg_q_len, seg_kv_len, reach, keep, k_out, v_out, out_table, out_stride, Hkv, D, err};
+    const dim3 grid(n, Hkv, 2);
+    if (dtype == KVB_BF16) {
+        if (store == KVB_E4M3) kvb_launch(expand_any_kernel<bf16, KVB_E4M3>, grid, dim3(256), 0, stream, p);
+        else kvb_launch(expand_any_kernel<bf16, KVB_INT8>, grid, dim3(256), 0, stream, p);
+    } else if (dtype == KVB_F32) {
+        if (store == KVB_E4M3) kvb_launch(expand_any_kernel<float, KVB_E4M3>, grid, dim3(256), 0, stream, p);
+        else kvb_launch(expand_any_kernel<float, KVB_INT8>, grid, dim3(256), 0, stream, p);
+    } else {
+        return KVB_ERR_DTYPE;
+    }
+    return kvb_launch_status();
+}
+
+// ---- attention, any size -----------------------------------------------------------------------------------------------------
+// One block per (row, query head); the running maximum and sum of csrc/attention_generic.cu over chunks of keys.
+#define QUANT_THREADS 128
+#define QUANT_MAX_D 1024
+struct AttendParams {
+    const void* q;
+    const uint8_t* k_codes;
+    const uint8_t* v_codes;
+    const uint8_t* k_scales;
+    const uint8_t* v_scales;
+    int num_pages;
+    const int* block_table;
+    int table_stride;
+    const int* positions;
+    const int* row_segment;
+    void* out;
+    int Hq, Hkv, D, page_size, reach, keep;
+    const float* sink;
+    const float* slopes;
+    float scale, cap;
+    int* err;
+};
+
+template <typename T, int STORE>
+__global__ void attention_quant_any_kernel(const AttendParams p) {
+    pdl_wait();
+    pdl_launch_dependents();
+    extern __shared__ float smem[];
+    const int D = p.D;
+    float* q_s = smem;                                      // [D]
+    float* p_s = q_s + D;                                   // [QUANT_THREADS]
+    long long* at_s = (long long*)(p_s + QUANT_THREADS + (D & 1));   // [QUANT_THREADS] the key's row among the pool's, -1: none
+    float* scratch = (float*)(at_s + QUANT_THREADS);        // [33]
+    const int r = blockIdx.x, h = blockIdx.y, hk = h / (p.Hq / p.Hkv);
+    const int pos = p.positions[r];
+    const int* table = p.block_table + (size_t)p.row_segment[r] * p.table_stride;
+    const int lo = first_seen_key(pos, p.reach), kept = min(p.reach > 0 ? p.keep : 0, lo), visible = kept + pos - lo + 1;
+    const T* qr = (const T*)p.q + ((size_t)r * p.Hq + h) * D;
+    for (int d = threadIdx.x; d < D; d += QUANT_THREADS) q_s[d] = to_f32<T>(qr[d]);
+    __syncthreads();
+    constexpr int DPT = QUANT_MAX_D / QUANT_THREADS;
+    float acc[DPT];
+#pragma unroll
+    for (int i = 0; i < DPT; ++i) acc[i] = 0.f;
+    float m = -FLT_MAX, l = 0.f;
+    if (p.sink) { m = p.sink[h]; l = 1.f; }
+    const float slope = p.slopes ? p.slopes[h] : 0.f;
+    for (int base = 0; base < visible; base += QUANT_THREADS) {
+        const int i = base + threadIdx.x, j = i < kept ? i : lo + (i - kept);
+        float s = -FLT_MAX;
+        long long at = -1;
+        if (i < visible) {
+            const int place = j / p.page_size, page = place < p.table_stride ? table[place] : -1;
+            if (page < 0 || page >= p.num_pages) {
+                atomicOr(p.err, KVB_DEV_BAD_PAGE);
+            } else {
+                at = ((long long)page * p.Hkv + hk) * p.page_size + j % p.page_size;
+                float dot = 0.f;
+                for (int d = 0; d < D; ++d) dot = fmaf(q_s[d], code_value<STORE>(p.k_codes[at * D + d]), dot);
+                s = dot * scale_up(p.k_scales[at]) * p.scale;
+                if (p.cap > 0.f) s = p.cap * tanhf(s / p.cap);
+                if (p.slopes) s -= slope * (float)(pos - j);
+            }
+        }
+        const float m_new = fmaxf(m, block_max(s, scratch));
+        const float corr = expf(m - m_new), weight = at >= 0 ? expf(s - m_new) : 0.f;
+        p_s[threadIdx.x] = at >= 0 ? weight * scale_up(p.v_scales[at]) : 0.f;
+        at_s[threadIdx.x] = at;
+        l = l * corr + block_sum(weight, scratch);          // also orders the writes to p_s and at_s
+        m = m_new;
+        const int n = min(QUANT_THREADS, visible - base);
+#pragma unroll
+        for (int i2 = 0; i2 < DPT; ++i2) {
+            const int d = threadIdx.x + i2 * QUANT_THREADS;
+            if (d < D) {
+                float a = acc[i2] * corr;
+                for (int t = 0; t < n; ++t)
+                    if (at_s[t] >= 0) a = fmaf(p_s[t], code_value<STORE>(p.v_codes[at_s[t] * D + d]), a);
+                acc[i2] = a;
+            }
+        }
+        __syncthreads();
+    }
+    T* out = (T*)p.out + ((size_t)r * p.Hq + h) * D;
+#pragma unroll
+    for (int i = 0; i < DPT; ++i) {
+        const int d = threadIdx.x + i * QUANT_THREADS;
+        if (d < D) out[d] = from_f32<T>(l == 0.f ? 0.f : acc[i] / l);
+    }
+}
+
+KVB_API int kvb_attention_quant_any(int dtype, int store, const void* q, const void* k_codes, const void* v_codes, const void* k_scales,
+                                    const void* v_scales, int num_pages, const int* block_table, int table_stride, const int* positions,
+                                    const int* row_segment, void* out, int T, int Hq, int Hkv, int D, int page_size, int reach, int keep,
+                                    const float* sink, const float* slopes, float cap, float scale, int* err, cudaStream_t stream) {
+    if (T <= 0) return KVB_OK;
+    if (store != KVB_E4M3 && store != KVB_INT8) return KVB_ERR_DTYPE;
+    if (D < 1 || D > QUANT_MAX_D || Hkv < 1 || Hq % Hkv != 0 || Hq > 65535 || page_size < 1 || num_pages < 1 || keep < 0 || cap < 0.f) return KVB_ERR_SHAPE;
+    const AttendParams p = {q, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scales, (const uint8_t*)v_scales, num_pages, block_table,
+                            table_stride, positions, row_segment, out, Hq, Hkv, D, page_size, reach, keep, sink, slopes, scale, cap, err};
+    const size_t smem = (size_t)(D + (D & 1) + QUANT_THREADS + 33) * 4 + QUANT_THREADS * 8;
+    const dim3 grid(T, Hq);
+    if (dtype == KVB_BF16) {
+        if (store == KVB_E4M3) kvb_launch(attention_quant_any_kernel<bf16, KVB_E4M3>, grid, dim3(QUANT_THREADS), smem, stream, p);
+        else kvb_launch(attention_quant_any_kernel<bf16, KVB_INT8>, grid, dim3(QUANT_THREADS), smem, stream, p);
+    } else if (dtype == KVB_F32) {
+        if (store == KVB_E4M3) kvb_launch(attention_quant_any_kernel<float, KVB_E4M3>, grid, dim3(QUANT_THREADS), smem, stream, p);
+        else kvb_launch(attention_quant_any_kernel<float, KVB_INT8>, grid, dim3(QUANT_THREADS), smem, stream, p);
+    } else {
+        return KVB_ERR_DTYPE;
+    }
+    return kvb_launch_status();
+}

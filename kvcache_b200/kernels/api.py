@@ -10,14 +10,16 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import dataclasses
 from collections import Counter
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
-from ..parts.base import PagedKVView, StepBatch
+from ..parts.base import STORE_DTYPES, PagedKVView, StepBatch, StepPlan
 from . import build
 from .attention_plan import PREFILL_MIN_KEY_TILES, TC_MAX_PAIRS, TC_MIN_KEY_TILES, TC_PAIR_MIN_KEY_TILES, PagedAttentionPlanner
+from .cache_plan import EXPAND_BLOCK, CacheExpandPlanner
 from .latent_plan import LatentAttentionPlanner, LatentExpandPlanner
 
 _c_int, _c_float, _c_void_p, _c_longlong = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong
@@ -174,6 +176,17 @@ _SIGNATURES = {
                                        _c_float, _c_void_p, _c_void_p, _c_void_p],
         "kvb_paged_attention_shared": [_c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p,
                                        _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_void_p],
+    },
+    "cache_quant": {
+        "kvb_append_quant": [_c_int, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_float, _c_void_p, _c_void_p, _c_int, _c_int,
+                             _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int,
+                             _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+        "kvb_cache_expand": [_c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int,
+                             _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p,
+                             _c_void_p],
+        "kvb_attention_quant_any": [_c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p,
+                                    _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_float,
+                                    _c_float, _c_void_p, _c_void_p],
     },
     "latent": {
         "kvb_norm_add_rmsnorm": [_c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_float, _c_void_p, _c_float, _c_void_p, _c_void_p,
@@ -333,6 +346,8 @@ class CudaKernels(KernelSet):
         self._rope = _Library("rope_append")
         self._attn_generic = _Library("attention_generic")
         self._gemm_simt = _Library("gemm_simt")
+        self._cache_quant = _Library("cache_quant")
+        self._expand_cache_planners: Dict[tuple, "CacheExpandPlanner"] = {}
         self._latent = _Library("latent")
         self._recurrent = _Library("recurrent")
         self._scan_wide = _Library("scan_wide")
@@ -616,6 +631,8 @@ class CudaKernels(KernelSet):
         16 j + 8 + i (i < 8) are dimensions 8 j + i and D / 2 + 8 j + i (see `pair_rotation_rows`)."""
         M, K = x16.shape
         spec = kv.spec
+        if spec.store is not None:
+            raise KernelError("the folded q/k/v projection writes caches in the compute type only")
         if cos is not None and cos.shape[1] * 2 != spec.head_dim:
             raise KernelError("the folded q/k/v projection rotates whole heads only")
         self._count("gemm_skinny_qkv")
@@ -818,9 +835,19 @@ class CudaKernels(KernelSet):
         `key_dim` numbers in `qkv` and are stored `kv.spec.head_dim` wide, with zeros after them.  `value_dim` <
         `kv.spec.v_head_dim`: likewise for the values.  `q_temperature` = (coef, every): the queries of a row at position p are
         multiplied by 1 + coef ln(floor((p + 1) / every) + 1).  `queries_only`: rows of queries alone, nothing is appended (a
-        layer that reads the cache entry of another)."""
+        layer that reads the cache entry of another).
+
+        Where `kv.spec.store` says so, keys and values are quantised from float32 into eight bits and one power of two a row
+        (csrc/cache_quant.cuh); bias, rotation and norms per head before it go with that."""
         T = qkv.shape[0]
         spec = kv.spec
+        if spec.store is not None:
+            plain = {"norm_scope": norm_scope == "head", "norm_after_rotation": not norm_after_rotation, "value_mix": value_mix is None,
+                     "q_temperature": q_temperature is None, "key_dim": key_dim in (None, spec.head_dim), "value_dim": value_dim in (None, spec.head_dim)}
+            if not all(plain.values()):
+                raise KernelError(f"qkv_rope_append: {', '.join(k for k, ok in plain.items() if not ok)} is not built for a cache in eight bits")
+            self._append_quantised(qkv, bias, cos, sin, batch, kv, q_out, num_heads, q_norm, k_norm, norm_eps, queries_only)
+            return
         rot_half = 0 if cos is None else cos.shape[1]
         table_len = 0 if cos is None else cos.shape[0]
         D = spec.head_dim if key_dim is None else int(key_dim)
@@ -851,6 +878,106 @@ class CudaKernels(KernelSet):
             _ptr(batch.positions), _ptr(batch.row_segment), _ptr(kv.block_table), kv.block_table.shape[1],
             _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(q_out), T, num_heads, spec.num_kv_heads, spec.head_dim,
             kv.page_size, 1 if kv.writes else 0, _ptr(self.error_word), self._stream()), "qkv_rope_append")
+
+    # ---- cache entries in eight bits -----------------------------------------------------------------------------------------
+    _STORE_CODES = {"e4m3": 0, "int8": 1}
+
+    def _quantised_entry(self, kv: PagedKVView, what: str) -> int:
+        """The store's code, after the checks of a view of such an entry."""
+        spec = kv.spec
+        dtype = STORE_DTYPES.get(spec.store)
+        if dtype is None:
+            raise KernelError(f"{what}: a cache is held as one of {', '.join(STORE_DTYPES)}, not '{spec.store}'")
+        if spec.v_head_dim != spec.head_dim:
+            raise KernelError(f"{what}: a cache in eight bits has values as wide as keys")
+        shape = (kv.k_pages.shape[0], spec.num_kv_heads, kv.page_size)
+        if kv.k_pages.dtype != dtype or kv.v_pages.dtype != dtype or kv.k_pages.shape != (*shape, spec.head_dim) or kv.v_pages.shape != kv.k_pages.shape:
+            raise KernelError(f"{what}: pages of a cache held as {spec.store} are {dtype} [pages, kv heads, page size, head size]")
+        for scales in (kv.k_scales, kv.v_scales):
+            if scales is None or scales.dtype != torch.uint8 or scales.shape != shape:
+                raise KernelError(f"{what}: a cache in eight bits has scale bytes, uint8 [pages, kv heads, page size]")
+        return self._STORE_CODES[spec.store]
+
+    def _append_quantised(self, qkv, bias, cos, sin, batch: StepBatch, kv: PagedKVView, q_out, num_heads: int, q_norm, k_norm, norm_eps: float,
+                          queries_only: bool) -> None:
+        spec = kv.spec
+        store = self._quantised_entry(kv, "qkv_rope_append")
+        T, D = qkv.shape[0], spec.head_dim
+        writes = kv.writes and not queries_only
+        if queries_only and kv.writes:
+            raise KernelError("qkv_rope_append: rows of queries alone, but the call writes the cache")
+        if (q_norm is None) != (k_norm is None) and not queries_only:
+            raise KernelError("qkv_rope_append: weights for the norms of queries and keys, or for neither")
+        if q_norm is not None and not norm_eps > 0.0:
+            raise KernelError("qkv_rope_append: a norm's eps is above zero")
+        width = (num_heads + (0 if queries_only else 2 * spec.num_kv_heads)) * D
+        if qkv.shape[1] < width or q_out.dtype != qkv.dtype or q_out.numel() != T * num_heads * D or (bias is not None and bias.numel() < width):
+            raise KernelError("qkv_rope_append: rows, biases or queries do not fit the heads")
+        self._count("append_quant")
+        _check(self._cache_quant.kvb_append_quant(
+            _dtype_code(qkv.dtype), store, _ptr(qkv), qkv.shape[1], _ptr(bias), _ptr(q_norm), _ptr(k_norm), float(norm_eps), _ptr(cos), _ptr(sin),
+            0 if cos is None else cos.shape[1], 0 if cos is None else cos.shape[0], _ptr(batch.positions), _ptr(batch.row_segment),
+            _ptr(kv.block_table), kv.block_table.shape[1], _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales),
+            kv.k_pages.shape[0], _ptr(q_out), T, num_heads, spec.num_kv_heads, D, kv.page_size, 1 if writes else 0, _ptr(self.error_word),
+            self._stream()), "qkv_rope_append")
+
+    def cache_expand_planner(self, reach: int = 0, keep_first: int = 0, singles: bool = True) -> CacheExpandPlanner:
+        """The lists `expand_cache` reads from `StepBatch.plans`, for layers that see `reach` (see parts.base.reach_code) and the first
+        `keep_first` keys.  `singles` False: requests that bring one token are left out (their attention reads the codes)."""
+        key = (int(reach), int(keep_first) if reach > 0 else 0, bool(singles))
+        found = self._expand_cache_planners.get(key)
+        if found is None:
+            found = self._expand_cache_planners[key] = CacheExpandPlanner(*key)
+        return found
+
+    def _expand_plan(self, batch: StepBatch, reach: int, keep: int):
+        for singles in (True, False):
+            plan = batch.plans.get(CacheExpandPlanner.plan_name(reach, keep if reach > 0 else 0, singles))
+            if plan is not None:
+                return plan, singles
+        return None, False
+
+    def expand_cache(self, batch: StepBatch, kv: PagedKVView, dtype: torch.dtype, workspace, reach: Optional[int] = None) -> PagedKVView:
+        """The keys and values that a step's rows see in a cache entry in eight bits, as float32 or bfloat16 (which holds them
+        exactly) in pages of 64 tokens that `paged_attention` takes: one page for every 64 keys of every request of the plan (see
+        `cache_expand_planner`), in order.  Keys behind a request's last, and before its rows' window, are zeros.  The pages lie in
+        the workspace and last until its next call."""
+        spec = kv.spec
+        reach = spec.reach if reach is None else int(reach)
+        store = self._quantised_entry(kv, "expand_cache")
+        plan, _ = self._expand_plan(batch, reach, spec.keep_first)
+        if plan is None:
+            raise KernelError("expand_cache: the step has no list of blocks (cache_expand_planner)")
+        n, S, D, Hkv = plan.counts["blocks"], batch.num_segments, spec.head_dim, spec.num_kv_heads
+        name = "f32" if dtype == torch.float32 else "bf16"
+        k_out = workspace.buffer(f"cache.expand_k_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
+        v_out = workspace.buffer(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
+        stride = -(-kv.block_table.shape[1] * kv.page_size // EXPAND_BLOCK)
+        table = workspace.buffer("cache.expand_table", (S, stride), torch.int32)
+        view = PagedKVView(dataclasses.replace(spec, store=None), k_out, v_out, table, EXPAND_BLOCK, False)
+        if n:
+            self._count("cache_expand")
+            _check(self._cache_quant.kvb_cache_expand(
+                _dtype_code(dtype), store, _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
+                _ptr(kv.block_table), kv.block_table.shape[1], kv.page_size, _ptr(plan.arrays["ranges"]), S, n, _ptr(batch.seg_q_len),
+                _ptr(batch.seg_kv_len), reach, spec.keep_first, _ptr(k_out), _ptr(v_out), _ptr(table), stride, Hkv, D, _ptr(self.error_word),
+                self._stream()), "expand_cache")
+        return view
+
+    def _quantised_attention(self, q, batch: StepBatch, kv: PagedKVView, out, num_heads: int, scale: float, workspace, sink, score_cap, slopes,
+                             reach: int) -> None:
+        """`paged_attention` over a cache entry in eight bits."""
+        spec = kv.spec
+        store = self._quantised_entry(kv, "paged_attention")
+        T, D, Hkv = q.shape[0], spec.head_dim, spec.num_kv_heads
+        if num_heads % Hkv or q.numel() != T * num_heads * D or out.numel() != q.numel() or out.dtype != q.dtype:
+            raise KernelError("paged_attention: queries and results do not fit the heads")
+        self._count("attention_quant_any")
+        _check(self._cache_quant.kvb_attention_quant_any(
+            _dtype_code(q.dtype), store, _ptr(q), _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
+            _ptr(kv.block_table), kv.block_table.shape[1], _ptr(batch.positions), _ptr(batch.row_segment), _ptr(out), T, num_heads, Hkv, D,
+            kv.page_size, reach, spec.keep_first, _ptr(sink), _ptr(slopes), float(score_cap or 0.0), float(scale), _ptr(self.error_word),
+            self._stream()), "paged_attention")
 
     def _tma_clusters(self, lib, head_dim: int, nsplit: int) -> int:
         key = (head_dim, nsplit)
@@ -891,7 +1018,7 @@ class CudaKernels(KernelSet):
         spec = kv.spec
         D, Hkv, n = spec.head_dim, spec.num_kv_heads, batch.num_segments
         plan = batch.plans.get(PagedAttentionPlanner.name)
-        if not (self.fused_rope_min_requests is not None and n >= self.fused_rope_min_requests
+        if not (spec.store is None and self.fused_rope_min_requests is not None and n >= self.fused_rope_min_requests
                 and self.flash_attention and qkv.dtype == torch.bfloat16 and kv.writes and plan is not None
                 and batch.num_tokens == n and plan.counts["decode_items"] == n and num_heads // Hkv <= 16
                 and self._tma_decode(D, kv) and (cos is None or cos.shape[1] <= D // 2)
@@ -947,6 +1074,9 @@ class CudaKernels(KernelSet):
         T = q.shape[0]
         spec = kv.spec
         reach = spec.reach if reach is None else int(reach)
+        if spec.store is not None:
+            self._quantised_attention(q, batch, kv, out, num_heads, scale, workspace, sink, score_cap, slopes, reach)
+            return
         D, Hkv = spec.head_dim, spec.num_kv_heads
         plan = batch.plans.get(PagedAttentionPlanner.name)
         keep = spec.keep_first if reach > 0 else 0

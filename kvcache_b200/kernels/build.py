@@ -50,6 +50,7 @@ MODULES: Dict[str, dict] = {
     "elementwise": {"src": "elementwise.cu", "deps": ["common.cuh"]},
     "rope_append": {"src": "rope_append.cu", "deps": ["common.cuh"]},
     "attention_generic": {"src": "attention_generic.cu", "deps": ["common.cuh"]},
+    "cache_quant": {"src": "cache_quant.cu", "deps": ["common.cuh", "cache_quant.cuh"]},
     "gemm_simt": {"src": "gemm_simt.cu", "deps": ["common.cuh"]},
     "latent": {"src": "latent.cu", "deps": ["common.cuh", "mma_tile.cuh"]},
     "recurrent": {"src": "recurrent.cu", "deps": ["common.cuh"]},

@@ -26,6 +26,7 @@ import torch
 from ..weights.loader import TensorSpec
 
 TORCH_DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32, "int32": torch.int32}
+STORE_DTYPES = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}      # what a cache entry in eight bits is held as
 
 
 def reach_code(window: Optional[int], chunk: Optional[int]) -> int:
@@ -63,6 +64,8 @@ class PagedKVSpec:
     # With a window: the request's first `keep_first` keys stay visible to every later query (and their pages stay held).
     keep_first: int = 0
     chunk: Optional[int] = None
+    # None: pages hold the compute type.  "e4m3" or "int8": eight bits a number and one power of two a row (csrc/cache_quant.cuh).
+    store: Optional[str] = None
 
     @property
     def reach(self) -> int:
@@ -91,6 +94,9 @@ class PagedKVView:
     block_table: torch.Tensor        # int32 [segments capacity, pages per request]; -1 where no page is held
     page_size: int
     writes: bool = True              # False: the call reads what another call wrote
+    # With `spec.store`: the rows' scale bytes, uint8 [pages, num_kv_heads, page_size]; pages are then torch.float8_e4m3fn or torch.int8.
+    k_scales: Optional[torch.Tensor] = None
+    v_scales: Optional[torch.Tensor] = None
 
 
 class StepPlanner:
