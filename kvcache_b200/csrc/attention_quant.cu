@@ -139,7 +139,6 @@ template <int STORE, bool HALF_ROWS>
 __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int RG = HALF_ROWS ? 1 : 2;                   // rows a lane has: g, and g + 8
-    constexpr int ROWS = 8 * RG;
     int* const first = reinterpret_cast<int*>(smem + WARPS * WARP_BYTES);     // [segments + 1] the line before each segment
     __shared__ int scan_s[WARPS + 1], ticket_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;

@@ -264,6 +264,13 @@ _SIGNATURES = {
                               _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p,
                               _c_int, _c_void_p, _c_float, _c_int, _c_void_p],
     },
+    "attention_quant": {
+        "kvb_attention_quant_blocks": [],
+        "kvb_attention_quant_max_segments": [],
+        "kvb_attention_quant": [_c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int,
+                                _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_float,
+                                _c_float, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p],
+    },
     "attention_tc": {
         "kvb_attention_tc_head_dim": [],
         "kvb_attention_tc": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p,
@@ -348,6 +355,7 @@ class CudaKernels(KernelSet):
         self._gemm_simt = _Library("gemm_simt")
         self._cache_quant = _Library("cache_quant")
         self._expand_cache_planners: Dict[tuple, "CacheExpandPlanner"] = {}
+        self._attn_quant: Dict[int, Tuple[_Library, int]] = {}
         self._latent = _Library("latent")
         self._recurrent = _Library("recurrent")
         self._scan_wide = _Library("scan_wide")
@@ -964,14 +972,67 @@ class CudaKernels(KernelSet):
                 self._stream()), "expand_cache")
         return view
 
+    QUANT_MAX_SEGMENTS = 4096
+    # Bytes of keys and values that a layer reads back for a step's portions; longer ones read the codes in place.
+    CACHE_EXPAND_MAX_BYTES = 1 << 30
+    quant_expand_min_rows = 64           # portions of at least this many tokens have their keys and values read back first
+    quant_min_units = 2                  # units of 128 keys a block of csrc/attention_quant.cu takes at least
+
+    def _quant_library(self, head_dim: int) -> Tuple[_Library, int]:
+        found = self._attn_quant.get(head_dim)
+        if found is None:
+            lib = _Library("attention_quant", f"d{head_dim}", [f"-DKVB_HEAD_DIM={head_dim}"])
+            found = self._attn_quant[head_dim] = (lib, int(lib.kvb_attention_quant_blocks()))
+        return found
+
     def _quantised_attention(self, q, batch: StepBatch, kv: PagedKVView, out, num_heads: int, scale: float, workspace, sink, score_cap, slopes,
                              reach: int) -> None:
         """`paged_attention` over a cache entry in eight bits."""
         spec = kv.spec
         store = self._quantised_entry(kv, "paged_attention")
-        T, D, Hkv = q.shape[0], spec.head_dim, spec.num_kv_heads
+        T, D, Hkv, S = q.shape[0], spec.head_dim, spec.num_kv_heads, batch.num_segments
         if num_heads % Hkv or q.numel() != T * num_heads * D or out.numel() != q.numel() or out.dtype != q.dtype:
             raise KernelError("paged_attention: queries and results do not fit the heads")
+        if T == 0:
+            return
+        group = num_heads // Hkv
+        # Codes read in place: bfloat16, four sizes of heads, pages of at least the four keys whose scale bytes are fetched together.
+        direct = (q.dtype == torch.bfloat16 and D in (32, 64, 96, 128) and kv.page_size >= 4 and workspace is not None
+                  and S <= self.QUANT_MAX_SEGMENTS and (q.data_ptr() | out.data_ptr() | kv.k_pages.data_ptr() | kv.v_pages.data_ptr()) % 16 == 0
+                  and (kv.k_scales.data_ptr() | kv.v_scales.data_ptr()) % 4 == 0)
+        # Read back first: portions of enough rows, and what the codes' own kernel does not take.
+        plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
+        paged = batch.plans.get(PagedAttentionPlanner.name)
+        singles = S if batch.max_q_len == 1 else S if paged is None else paged.counts["decode_items"]
+        expand = (plan is not None and plan.counts["blocks"] > 0 and paged is not None and workspace is not None
+                  and 4 * plan.counts["blocks"] * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES)
+        if direct:
+            # Segments of single tokens keep to their codes; the portions' kernels have to leave them out.
+            expand = expand and batch.max_q_len >= self.quant_expand_min_rows and D % 16 == 0 and group <= 16
+        else:
+            expand = expand and (with_singles or singles == 0)
+        if expand:
+            view = self.expand_cache(batch, kv, q.dtype, workspace, reach)
+            portions = batch
+            if direct and singles:
+                portions = dataclasses.replace(batch, plans={**batch.plans, PagedAttentionPlanner.name: StepPlan(
+                    paged.arrays, {**paged.counts, "decode_items": 0})})
+            self.paged_attention(q, portions, view, out, num_heads, scale, workspace, sink=sink, score_cap=score_cap, slopes=slopes, reach=reach)
+            if not direct or not singles:
+                return
+        if direct:
+            lib, per_sm = self._quant_library(D)
+            most = 1 if expand else batch.max_q_len
+            blocks = min(per_sm * self.sm_count, S * Hkv * -(-most * group // 16) * (kv.block_table.shape[1] * kv.page_size // 128 + 3))
+            scratch = workspace.buffer("attn.quant_scratch", (2 * per_sm * self.sm_count * 16 * (D + 2),), torch.float32)
+            tickets = workspace.zeros("attn.quant_tickets", (per_sm * self.sm_count,), torch.int32)
+            self._count("attention_quant")
+            _check(lib.kvb_attention_quant(
+                store, _ptr(q), _ptr(out), _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
+                _ptr(kv.block_table), kv.block_table.shape[1], S, T, _ptr(batch.seg_q_start), _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len), most,
+                num_heads, Hkv, kv.page_size, reach, spec.keep_first, _ptr(sink), _ptr(slopes), float(score_cap or 0.0), float(scale),
+                _ptr(scratch), _ptr(tickets), blocks, self.quant_min_units, _ptr(self.error_word), self._stream()), "paged_attention")
+            return
         self._count("attention_quant_any")
         _check(self._cache_quant.kvb_attention_quant_any(
             _dtype_code(q.dtype), store, _ptr(q), _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
