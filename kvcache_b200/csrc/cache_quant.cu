@@ -9,8 +9,10 @@ using namespace cq;
 // ---- append ------------------------------------------------------------------------------------------------------------------
 // Rows of `qkv` are [Hq heads | Hkv key heads | Hkv value heads | ...] of D numbers, `row_stride` apart.  A query or key head x
 // becomes x / sqrt(mean(x^2) + eps) * w (eps > 0; w: D numbers or null), then its first 2 rot_half numbers are turned by the
-// row's angles as pairs (t, t + rot_half); queries are rounded to q_out, keys and values quantised from float32 - one rounding - into
-// the page of the row's position.  The scale needs the whole row's largest magnitude before the first code is written.
+// row's angles as pairs (t, t + rot_half); queries are rounded to q_out, keys and values quantised into the page of the row's position.
+// Keys and values are made in float64 from the inputs (a few operations a number, of rows that are few beside the queries): a code
+// is the rounding of the definition's number, whichever kernel writes it, and not of a float32 that lies beside a border.  The scale
+// needs the whole row's largest magnitude before the first code is written.
 struct AppendParams {
     const void* qkv;
     int row_stride;
@@ -46,7 +48,44 @@ __device__ __forceinline__ long long slot_of(const AppendParams& p, int row, int
     return (long long)page * p.Hkv * p.page_size + pos % p.page_size;
 }
 
-// Any head size, float32 or bfloat16: a warp a (row, head).  A number is made twice, for the largest and for its code.
+// Whether the row's angles are in the table; they are set to the first row's otherwise.
+__device__ __forceinline__ size_t angles_of(const AppendParams& p, int pos, bool report) {
+    const bool ok = p.rot_half == 0 || (pos >= 0 && pos < p.table_len);
+    if (!ok && report) atomicOr(p.err, KVB_DEV_BAD_POS);
+    return (size_t)(ok ? pos : 0) * p.rot_half;
+}
+
+// Any head size, float32 or bfloat16: a warp a (row, head).  A number is made twice, for the largest and for its code.  F: what the numbers
+// are made in.
+template <typename F, typename T>
+struct HeadNumbers {
+    const T* x;
+    const float* bias;
+    const float* weight;
+    const float* cr;
+    const float* sr;
+    int rot_half;
+    bool normed;
+    F inv;
+    __device__ __forceinline__ F biased(int d) const { return (F)to_f32<T>(x[d]) + (bias ? (F)bias[d] : (F)0); }
+    __device__ __forceinline__ F scaled(int d) const { const F v = biased(d); return normed ? (weight ? v * inv * (F)weight[d] : v * inv) : v; }
+    __device__ __forceinline__ F at(int d) const {
+        const F v = scaled(d);
+        if (d >= 2 * rot_half) return v;
+        const bool low = d < rot_half;
+        const int t = low ? d : d - rot_half;
+        const F partner = scaled(low ? d + rot_half : t);
+        return low ? v * (F)cr[t] - partner * (F)sr[t] : v * (F)cr[t] + partner * (F)sr[t];
+    }
+    __device__ __forceinline__ void norm(int D, float eps, int lane) {
+        F sum = 0;
+        for (int d = lane; d < D; d += 32) { const F v = biased(d); sum += v * v; }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        inv = (F)1 / sqrt(sum / (F)D + (F)eps);
+    }
+};
+
 template <typename T, int STORE>
 __global__ void append_quant_any_kernel(const AppendParams p) {
     pdl_wait();
@@ -59,44 +98,153 @@ __global__ void append_quant_any_kernel(const AppendParams p) {
     const bool is_q = head < p.Hq, is_v = head >= p.Hq + p.Hkv;
     const T* x = (const T*)p.qkv + (size_t)row * p.row_stride + (size_t)head * D;
     const float* bias = p.bias ? p.bias + (size_t)head * D : nullptr;
-    const float* weight = is_q ? p.q_norm : p.k_norm;
-    auto biased = [&](int d) { return to_f32<T>(x[d]) + (bias ? bias[d] : 0.f); };
-    float inv = 1.f;
-    if (!is_v && p.eps > 0.f) {
-        float sum = 0.f;
-        for (int d = lane; d < D; d += 32) { const float v = biased(d); sum = fmaf(v, v, sum); }
-        inv = rsqrtf(warp_sum(sum) / D + p.eps);
-    }
+    const size_t angle = angles_of(p, pos, lane == 0);
     const bool normed = !is_v && p.eps > 0.f;
-    auto scaled = [&](int d) { const float v = biased(d); return normed ? (weight ? v * inv * weight[d] : v * inv) : v; };
-    const bool pos_ok = p.rot_half == 0 || (pos >= 0 && pos < p.table_len);
-    if (!pos_ok && lane == 0) atomicOr(p.err, KVB_DEV_BAD_POS);
-    const float* cr = p.cos_t + (size_t)(pos_ok ? pos : 0) * p.rot_half;
-    const float* sr = p.sin_t + (size_t)(pos_ok ? pos : 0) * p.rot_half;
-    auto value = [&](int d) {
-        const float v = scaled(d);
-        if (is_v || d >= 2 * p.rot_half) return v;
-        const bool low = d < p.rot_half;
-        const int t = low ? d : d - p.rot_half;
-        const float partner = scaled(low ? d + p.rot_half : t);
-        return low ? v * cr[t] - partner * sr[t] : v * cr[t] + partner * sr[t];
-    };
     if (is_q) {
+        HeadNumbers<float, T> h = {x, bias, p.q_norm, p.cos_t + angle, p.sin_t + angle, p.rot_half, normed, 1.f};
+        if (normed) h.norm(D, p.eps, lane);
         T* out = (T*)p.q_out + ((size_t)row * p.Hq + head) * D;
-        for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(value(d));
+        for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(h.at(d));
         return;
     }
+    HeadNumbers<double, T> h = {x, bias, p.k_norm, p.cos_t + angle, p.sin_t + angle, is_v ? 0 : p.rot_half, normed, 1.0};
+    if (normed) h.norm(D, p.eps, lane);
     const long long slot = slot_of(p, row, pos, lane == 0);
     if (slot < 0) return;
     uint32_t top = 0u;
-    for (int d = lane; d < D; d += 32) top = max(top, __float_as_uint(value(d)) & 0x7fffffffu);
+    for (int d = lane; d < D; d += 32) top = max(top, __float_as_uint(__double2float_ru(fabs(h.at(d)))));
     top = __reduce_max_sync(0xffffffffu, top);
     const int byte = scale_byte<STORE>(top);
     const float down = scale_down(byte);
     const long long at = slot + (long long)(is_v ? head - p.Hq - p.Hkv : head - p.Hq) * p.page_size;
     uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + at * D;
-    for (int d = lane; d < D; d += 32) codes[d] = (uint8_t)code_of<STORE>(value(d), down);
+    for (int d = lane; d < D; d += 32) codes[d] = (uint8_t)code_of<STORE>(h.at(d), down);
     if (lane == 0) (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)byte;
+}
+
+// bfloat16, heads of 8 LANES numbers, rotated halves in steps of eight: LANES lanes hold a head, eight neighbouring numbers each, and a
+// rotation partner is some lanes away.  A block takes a row; its groups of lanes go through the row's heads with the same
+// place in each, so that a row's angles are read once.
+// Bound by bytes in long prompts: 2,048 rows of 36 heads of 128 (34 MB in and out) take APPEND_US, a warp a head with a number a lane 47 us.
+template <int LANES, int STORE, bool NORM>
+__global__ void __launch_bounds__(256) append_quant_vec_kernel(const AppendParams p) {
+    constexpr int D = 8 * LANES;
+    // The row's metadata, tables and biases are older than the product before this kernel.
+    const int row = blockIdx.x, lane = threadIdx.x & 31, li = lane & (LANES - 1), d = 8 * li;
+    const uint32_t group_mask = (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u) << (lane & ~(LANES - 1));
+    const int groups = blockDim.x / LANES, heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0);
+    const int pos = p.positions[row], rot = 2 * p.rot_half;
+    const size_t angle = angles_of(p, pos, threadIdx.x == 0);
+    const long long slot = p.write_kv ? slot_of(p, row, pos, threadIdx.x == 0) : -1;
+    const bool rotated = d < rot, low = d < p.rot_half;
+    const int partner = (lane & ~(LANES - 1)) + (rotated ? (low ? d + p.rot_half : d - p.rot_half) / 8 : li);
+    float cs[8], sn[8];
+    if (rotated) {
+        const size_t t = angle + (low ? d : d - p.rot_half);
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(p.cos_t + t + k), s = *reinterpret_cast<const float4*>(p.sin_t + t + k);
+            cs[k] = c.x; cs[k + 1] = c.y; cs[k + 2] = c.z; cs[k + 3] = c.w;
+            sn[k] = low ? -s.x : s.x; sn[k + 1] = low ? -s.y : s.y; sn[k + 2] = low ? -s.z : s.z; sn[k + 3] = low ? -s.w : s.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { cs[k] = 1.f; sn[k] = 0.f; }
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    const bf16* const rows = (const bf16*)p.qkv + (size_t)row * p.row_stride;
+    for (int head = threadIdx.x / LANES; head < heads; head += groups) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(rows + (size_t)head * D + d);
+        const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+        float b[8], w[8];
+        const bool is_q = head < p.Hq, is_v = head >= p.Hq + p.Hkv;
+        auto load8 = [](const float* from, float* to) {
+            const float4 x = *reinterpret_cast<const float4*>(from), y = *reinterpret_cast<const float4*>(from + 4);
+            to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w; to[4] = y.x; to[5] = y.y; to[6] = y.z; to[7] = y.w;
+        };
+        if (p.bias) load8(p.bias + (size_t)head * D + d, b);
+        const float* const weight = is_q ? p.q_norm : p.k_norm;
+        if (NORM && !is_v && weight) load8(weight + d, w);
+        auto number = [&](int k) { return __uint_as_float(k & 1 ? word[k >> 1] & 0xffff0000u : word[k >> 1] << 16); };
+        if (is_q) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = p.bias ? number(k) + b[k] : number(k);
+            if (NORM) {
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum = fmaf(x[k], x[k], sum);
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(group_mask, sum, o);
+                const float inv = 1.f / sqrtf(sum / D + p.eps);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = weight ? x[k] * inv * w[k] : x[k] * inv;
+            }
+            uint32_t out[4];
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+                const float a0 = __shfl_sync(group_mask, x[k], partner), a1 = __shfl_sync(group_mask, x[k + 1], partner);
+                __nv_bfloat162 y = rotated ? __floats2bfloat162_rn(fmaf(x[k], cs[k], a0 * sn[k]), fmaf(x[k + 1], cs[k + 1], a1 * sn[k + 1]))
+                                           : __floats2bfloat162_rn(x[k], x[k + 1]);
+                out[k >> 1] = *reinterpret_cast<uint32_t*>(&y);
+            }
+            *reinterpret_cast<uint4*>((bf16*)p.q_out + ((size_t)row * p.Hq + head) * D + d) = make_uint4(out[0], out[1], out[2], out[3]);
+            continue;
+        }
+        double x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = p.bias ? (double)number(k) + (double)b[k] : (double)number(k);
+        if (!is_v) {
+            if (NORM) {
+                double sum = 0.0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += x[k] * x[k];
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(group_mask, sum, o);
+                const double inv = 1.0 / sqrt(sum / D + (double)p.eps);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = weight ? x[k] * inv * (double)w[k] : x[k] * inv;
+            }
+            if (rot) {
+                double y[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = __shfl_sync(group_mask, x[k], partner);
+                if (rotated)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = x[k] * (double)cs[k] + y[k] * (double)sn[k];
+            }
+        }
+        uint32_t top = 0u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(__double2float_ru(fabs(x[k]))));
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(group_mask, top, o));
+        if (slot < 0) continue;
+        const int byte = scale_byte<STORE>(top);
+        const float down = scale_down(byte);
+        uint32_t codes[2] = {0u, 0u};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) codes[k >> 2] |= code_of<STORE>(x[k], down) << (8 * (k & 3));
+        const long long at = slot + (long long)(is_v ? head - p.Hq - p.Hkv : head - p.Hq) * p.page_size;
+        *reinterpret_cast<uint2*>((is_v ? p.v_codes : p.k_codes) + at * D + d) = make_uint2(codes[0], codes[1]);
+        if (li == 0) (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)byte;
+    }
+}
+
+template <int LANES>
+static int append_vec(const AppendParams& p, int store, cudaStream_t stream) {
+    // A group of lanes a head while rows are few (one row of 18 heads: a pass), half as many groups where rows fill the SMs anyway.
+    const int heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), wanted = (heads * LANES + 31) / 32 * 32;
+    const dim3 grid(p.T), block(wanted < 256 ? wanted : p.T >= 1024 && wanted >= 128 ? 128 : 256);
+    if (store == KVB_E4M3) {
+        if (p.eps > 0.f) kvb_launch(append_quant_vec_kernel<LANES, KVB_E4M3, true>, grid, block, 0, stream, p);
+        else kvb_launch(append_quant_vec_kernel<LANES, KVB_E4M3, false>, grid, block, 0, stream, p);
+    } else {
+        if (p.eps > 0.f) kvb_launch(append_quant_vec_kernel<LANES, KVB_INT8, true>, grid, block, 0, stream, p);
+        else kvb_launch(append_quant_vec_kernel<LANES, KVB_INT8, false>, grid, block, 0, stream, p);
+    }
+    return kvb_launch_status();
 }
 
 template <typename T>
@@ -122,6 +270,14 @@ KVB_API int kvb_append_quant(int dtype, int store, const void* qkv, int row_stri
     const AppendParams p = {qkv, row_stride, bias, q_norm, k_norm, eps, cos_t, sin_t, rot_half, table_len, positions, row_segment, block_table,
                             table_stride, (uint8_t*)k_codes, (uint8_t*)v_codes, (uint8_t*)k_scales, (uint8_t*)v_scales, num_pages, q_out, T, Hq, Hkv, D,
                             page_size, write_kv, err};
+    const uintptr_t addresses = (uintptr_t)qkv | (uintptr_t)bias | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos_t | (uintptr_t)sin_t |
+                                (uintptr_t)q_out | (uintptr_t)k_codes | (uintptr_t)v_codes;
+    if (dtype == KVB_BF16 && (addresses & 15) == 0 && row_stride % 8 == 0 && rot_half % 8 == 0) {
+        if (D == 64) return append_vec<8>(p, store, stream);
+        if (D == 128) return append_vec<16>(p, store, stream);
+        if (D == 32) return append_vec<4>(p, store, stream);
+        if (D == 256) return append_vec<32>(p, store, stream);
+    }
     if (dtype == KVB_BF16) return append_any<bf16>(p, store, stream);
     if (dtype == KVB_F32) return append_any<float>(p, store, stream);
     return KVB_ERR_DTYPE;
@@ -191,6 +347,87 @@ __global__ void expand_any_kernel(const ExpandParams p) {
     }
 }
 
+// Heads in steps of eight numbers: a thread reads eight codes and writes eight numbers, four at a time in flight.
+template <typename T> __device__ __forceinline__ void store8(T* to, const float* x);
+template <> __device__ __forceinline__ void store8<float>(float* to, const float* x) {
+    *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <> __device__ __forceinline__ void store8<bf16>(bf16* to, const float* x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        __nv_bfloat162 y = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+        w[k] = *reinterpret_cast<uint32_t*>(&y);
+    }
+    *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T, int STORE>
+__global__ void __launch_bounds__(256) expand_vec_kernel(const ExpandParams p) {
+    const int i = blockIdx.x, hk = blockIdx.y, D = p.D, chunks = D >> 3;
+    const bool values = blockIdx.z == 1;
+    int seg, block;
+    find_block(p, i, seg, block);
+    const int kv_len = p.seg_kv_len[seg], lo = first_seen_key(kv_len - p.seg_q_len[seg], p.reach), keep = p.reach > 0 ? p.keep : 0;
+    const int* const table = p.block_table + (size_t)seg * p.table_stride;
+    const uint8_t* const codes = values ? p.v_codes : p.k_codes;
+    const uint8_t* const scales = values ? p.v_scales : p.k_scales;
+    T* const out = (T*)(values ? p.v_out : p.k_out) + ((size_t)i * p.Hkv + hk) * READ_BLOCK * D;
+    constexpr int FLIGHT = 4;
+    bool waited = false;
+    for (int c0 = threadIdx.x; c0 < READ_BLOCK * chunks; c0 += FLIGHT * 256) {
+        long long at[FLIGHT];
+        uint2 code[FLIGHT];
+        int byte[FLIGHT];
+#pragma unroll
+        for (int f = 0; f < FLIGHT; ++f) {
+            const int c = c0 + f * 256, r = c / chunks, key = block * READ_BLOCK + r;
+            at[f] = -1;
+            if (c < READ_BLOCK * chunks && key < kv_len && (key >= lo || key < keep)) {
+                const int place = key / p.page_size;
+                const int page = place < p.table_stride ? table[place] : -1;
+                if (page >= 0 && page < p.num_pages) at[f] = ((long long)page * p.Hkv + hk) * p.page_size + key % p.page_size;
+                else atomicOr(p.err, KVB_DEV_BAD_PAGE);
+            }
+        }
+        if (!waited) {                                       // up to here only what the step brought along
+            waited = true;
+            pdl_wait();
+            pdl_launch_dependents();
+            if (hk == 0 && !values && threadIdx.x == 0 && block < p.out_stride) p.out_table[(size_t)seg * p.out_stride + block] = i;
+        }
+#pragma unroll
+        for (int f = 0; f < FLIGHT; ++f) {
+            code[f] = make_uint2(0u, 0u);
+            byte[f] = 0;
+            if (at[f] >= 0) {
+                code[f] = *reinterpret_cast<const uint2*>(codes + at[f] * D + ((c0 + f * 256) % chunks) * 8);
+                byte[f] = scales[at[f]];
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < FLIGHT; ++f) {
+            const int c = c0 + f * 256;
+            if (c >= READ_BLOCK * chunks) break;
+            const float up = at[f] >= 0 ? scale_up(byte[f]) : 0.f;
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = code_value<STORE>(((k < 4 ? code[f].x : code[f].y) >> (8 * (k & 3))) & 255u) * up;
+            store8<T>(out + (size_t)c * 8, x);
+        }
+    }
+}
+
+template <typename T>
+static int expand(const ExpandParams& p, int store, int n, cudaStream_t stream) {
+    const dim3 grid(n, p.Hkv, 2);
+    const bool vec = p.D % 8 == 0 && (((uintptr_t)p.k_codes | (uintptr_t)p.v_codes) & 7) == 0 && (((uintptr_t)p.k_out | (uintptr_t)p.v_out) & 15) == 0;
+    if (store == KVB_E4M3) kvb_launch(vec ? expand_vec_kernel<T, KVB_E4M3> : expand_any_kernel<T, KVB_E4M3>, grid, dim3(256), 0, stream, p);
+    else kvb_launch(vec ? expand_vec_kernel<T, KVB_INT8> : expand_any_kernel<T, KVB_INT8>, grid, dim3(256), 0, stream, p);
+    return kvb_launch_status();
+}
+
 KVB_API int kvb_cache_expand(int dtype, int store, const void* k_codes, const void* v_codes, const void* k_scales, const void* v_scales, int num_pages,
                              const int* block_table, int table_stride, int page_size, const int* ranges, int segments, int n,
                              const int* seg_q_len, const int* seg_kv_len, int reach, int keep, void* k_out, void* v_out, int* out_table, int out_stride, int Hkv, int D,
@@ -200,17 +437,9 @@ KVB_API int kvb_cache_expand(int dtype, int store, const void* k_codes, const vo
     if (D < 1 || Hkv < 1 || Hkv > 65535 || page_size < 1 || num_pages < 1 || keep < 0 || segments < 1) return KVB_ERR_SHAPE;
     const ExpandParams p = {(const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scales, (const uint8_t*)v_scales, num_pages, block_table,
                             table_stride, page_size, ranges, segments, seg_q_len, seg_kv_len, reach, keep, k_out, v_out, out_table, out_stride, Hkv, D, err};
-    const dim3 grid(n, Hkv, 2);
-    if (dtype == KVB_BF16) {
-        if (store == KVB_E4M3) kvb_launch(expand_any_kernel<bf16, KVB_E4M3>, grid, dim3(256), 0, stream, p);
-        else kvb_launch(expand_any_kernel<bf16, KVB_INT8>, grid, dim3(256), 0, stream, p);
-    } else if (dtype == KVB_F32) {
-        if (store == KVB_E4M3) kvb_launch(expand_any_kernel<float, KVB_E4M3>, grid, dim3(256), 0, stream, p);
-        else kvb_launch(expand_any_kernel<float, KVB_INT8>, grid, dim3(256), 0, stream, p);
-    } else {
-        return KVB_ERR_DTYPE;
-    }
-    return kvb_launch_status();
+    if (dtype == KVB_BF16) return expand<bf16>(p, store, n, stream);
+    if (dtype == KVB_F32) return expand<float>(p, store, n, stream);
+    return KVB_ERR_DTYPE;
 }
 
 // ---- attention, any size -----------------------------------------------------------------------------------------------------

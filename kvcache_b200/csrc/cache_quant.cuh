@@ -34,13 +34,14 @@ __device__ __forceinline__ int scale_byte(uint32_t top) {
 __device__ __forceinline__ float scale_down(int byte) { return byte == NOT_FINITE ? 0.f : __int_as_float((2 * BIAS - byte) << 23); }
 __device__ __forceinline__ float scale_up(int byte) { return __int_as_float(byte == NOT_FINITE ? 0x7fffffff : byte << 23); }
 
-// The code of x 2^-e, in the low byte.
+// The code of x 2^-e, in the low byte, rounded once: on the way to e4m3 a float32 that keeps a last bit of what it leaves out.
 template <int STORE>
-__device__ __forceinline__ uint32_t code_of(float x, float down) {
+__device__ __forceinline__ uint32_t code_of(double x, float down) {
     if (down == 0.f) return 0u;                       // x may be an infinity or NaN
-    const float y = x * down;
-    if (STORE == KVB_E4M3) return (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-    return (uint32_t)min(127, max(-127, __float2int_rn(y))) & 0xffu;
+    const double y = x * (double)down;
+    if (STORE == KVB_INT8) return (uint32_t)min(127, max(-127, __double2int_rn(y))) & 0xffu;
+    const float f = __double2float_rz(y);
+    return (uint32_t)__nv_cvt_float_to_fp8((double)f == y ? f : __uint_as_float(__float_as_uint(f) | 1u), __NV_SATFINITE, __NV_E4M3);
 }
 template <int STORE>
 __device__ __forceinline__ float code_value(uint32_t code) {
