@@ -7,18 +7,22 @@
 // with (c, e) a key's and (d, f) a value's row.  The weights that meet the value codes are n_j = 2^(score_j log2 e + f_j - m), m the
 // largest of those exponents so far: at most 1, and what matters for the sum is near 1 whatever the rows' scales are, so that half
 // precision holds them to 2^-11.  The denominator takes n_j 2^(-f_j), in float32.  Codes are exact in half precision, and so
-// are queries once a power of two has brought their row to about 1: products run on mma.sync m16n8k16 (half, float32 sums),
-// whose 16 rows are the query heads that share a key head (times the tokens of a short portion).
+// are queries once a power of two has brought their row to about 1: products run on mma.sync m16n8k16 (half, float32 sums).
 //
-// A warp takes 32 keys at a time and needs nothing from any other until its run ends.  The order of an MMA's inner index is free as
-// long as both operands agree, so a lane's share of a tile is bytes that lie together: for the scores 16 (or 8) of a key's
+// Codes are the operand with 16 rows, S^T = K Q^T and O^T = V^T P^T, so that eight query rows - the heads that share a key head,
+// times the tokens of a short portion - fill an MMA, and what a code costs on its way to half precision is paid once for up to
+// ROW_TILES eights of rows.  (Queries as the 16 rows: twice the MMAs and sums in registers for seven heads.)
+// A warp takes 32 keys at a time and needs nothing from any other until its run ends.  The order of an MMA's inner index, and of its
+// rows, is free as long as all agree, so a lane's share of a tile is bytes that lie together: for the scores 16 (or 8) of a key's
 // numbers, for the sum the same of four neighbouring keys' values.  Each lane copies those bytes itself (cp.async, into slots of
-// shared memory that no other lane touches), several tiles ahead, and turns them into half precision in registers: no barrier, no
+// shared memory that no other lane touches), a tile ahead, and turns them into half precision in registers: no barrier, no
 // bank conflict and no wait for another lane stands in the stream.
 //
-// Work is shared out by keys: units of 128 keys of every (segment, key head, tile of 16 rows), laid end to end, are cut into equal
+// Work is shared out by keys: units of 128 keys of every (segment, key head, tile of rows), laid end to end, are cut into equal
 // runs, one a block, whatever the lengths.  Where a cut divides a row tile's keys, the pieces' sums meet in scratch, two places a
-// block, and the last piece to finish adds them in order (a ticket per block): the same bits whichever is last.
+// block: the last of eight neighbours to finish adds them in order, and so on up to the whole: the same bits whichever is last, and
+// none of many pieces waits for one block to read them all (131,072 keys of 4 heads in 103 pieces each: 74 us with one
+// block adding all).
 #include "cache_quant.cuh"
 #include <type_traits>
 
@@ -36,12 +40,13 @@ constexpr int WARP_KEYS = 32, UNIT = WARPS * WARP_KEYS;
 constexpr int KU = D % 64 == 0 ? 16 : 8, KN = D / (4 * KU);                       // bytes a copy, copies a key row and lane: four lanes share a key row
 constexpr int VU = D % 128 == 0 ? 16 : D % 64 == 0 ? 8 : 4, VN = D / (8 * VU);    // ... eight lanes share a value row
 constexpr int K_BYTES = 4 * KN * KU * 32, V_BYTES = 8 * VN * VU * 32, STAGE_BYTES = K_BYTES + V_BYTES + 4 * 32 * 4;
-constexpr int STAGES = D == 128 ? 3 : 4;
+constexpr int STAGES = 2;
 constexpr int WARP_BYTES = STAGES * STAGE_BYTES;
 constexpr int O_STRIDE = D + 4;
-constexpr int BLOCKS_PER_SM = D == 128 ? 2 : D == 96 ? 2 : 3;
-static_assert(16 * O_STRIDE * 4 + 128 <= WARP_BYTES, "a warp's sums lie over its slots");
+// Blocks an SM holds of the kernel for ROW_TILES eights of rows: registers allow 3 of 168 a thread, or 4 of 128, or 2 of 255.
+template <int ROW_TILES> constexpr int blocks_per_sm() { return ROW_TILES == 1 ? (D <= 64 ? 4 : 3) : ROW_TILES == 2 ? (D <= 64 ? 3 : 2) : 2; }
 constexpr int MAX_SEGMENTS = 4096;
+constexpr int GROUP = 8;               // pieces whose sums one block adds up
 constexpr int PIECE_COST = 1;          // what a piece costs beside its keys, in units
 constexpr float NEG_INF = -INFINITY;
 
@@ -64,9 +69,9 @@ struct Params {
     float scale, cap;
     const float* sink;
     const float* slopes;
-    float* part_o;             // [2 * blocks, 16, D]
-    float* part_ml;            // [2 * blocks, 16, 2]
-    int* tickets;              // [blocks], zero between launches
+    float* part_o;             // [2 * blocks, rows of a tile, D]
+    float* part_ml;            // [2 * blocks, rows of a tile, 2]
+    int* tickets;              // [7 * blocks], zero between launches
     int min_units;
     int* err;
 };
@@ -89,26 +94,33 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// c += a b; rows 8 to 15 of a are zero where HALF_ROWS.
-template <bool HALF_ROWS>
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(HALF_ROWS ? 0u : a[1]), "r"(a[HALF_ROWS ? 1 : 2]), "r"(HALF_ROWS ? 0u : a[3]), "r"(b0), "r"(b1));
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
-// Two neighbouring codes of a word (the lower or the upper two bytes) as half precision.  int8: the bytes, with their sign bits
-// flipped (`flipped`), become the low bits of 1024 + c + 128, from which 1152 is taken.
-template <int STORE> __device__ __forceinline__ uint32_t flipped(uint32_t w) { return STORE == KVB_INT8 ? w ^ 0x80808080u : w; }
-template <int STORE, int UPPER>
-__device__ __forceinline__ uint32_t halves(uint32_t w) {
+// The 8 x 8 matrix of 16-bit numbers that a warp holds, a row a group of four lanes, turned.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+// A word of four codes as half precision: its bytes 0 and 2, and its bytes 1 and 3.  An e4m3 number's exponent and mantissa are put where
+// half precision has them, which makes it 2^-8 times as large (CODE_SCALE), subnormal ones included: seven instructions, where
+// the conversion instruction takes fourteen for four codes.  An int8 code with its sign bit flipped becomes the low bits of 1024 + c + 128.
+template <int STORE>
+__device__ __forceinline__ void halves(uint32_t w, uint32_t& even, uint32_t& odd) {
     if (STORE == KVB_INT8) {
-        const uint32_t v = __byte_perm(w, 0x64646464u, UPPER ? 0x4342 : 0x4140);
-        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&v), __half2half2(__ushort_as_half(0x6480)));
-        return *reinterpret_cast<const uint32_t*>(&h);
+        const __half2 off = __half2half2(__ushort_as_half(0x6480));          // 1152
+        const uint32_t a = (w & 0x00ff00ffu) ^ 0x64806480u, b = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+        even = *reinterpret_cast<const uint32_t*>(&x);
+        odd = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+        even = ((w << 7) & 0x3f803f80u) | ((w << 8) & 0x80008000u);
+        odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
     }
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(UPPER ? w >> 16 : w & 0xffffu), __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
 }
+template <int STORE> constexpr float CODE_SCALE = STORE == KVB_E4M3 ? 256.f : 1.f;
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -120,6 +132,7 @@ struct Segment {
     int tile_begin, n_keep, n;         // the list of units: n_keep units of kept keys, then from unit tile_begin on
     int row_tiles;
 };
+template <int ROWS>
 __device__ __forceinline__ Segment make_segment(const Params& p, int s) {
     Segment c;
     c.q_start = p.seg_q_start[s];
@@ -131,14 +144,15 @@ __device__ __forceinline__ Segment make_segment(const Params& p, int s) {
     c.tile_begin = first_seen_key(c.start, p.reach) / UNIT;
     c.n_keep = min((c.keep + UNIT - 1) / UNIT, c.tile_begin);
     c.n = c.n_keep + (kv_len - 1) / UNIT + 1 - c.tile_begin;
-    c.row_tiles = (c.q_len * p.group + 15) >> 4;
+    c.row_tiles = (c.q_len * p.group + ROWS - 1) / ROWS;
     return c;
 }
 
-template <int STORE, bool HALF_ROWS>
-__global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel(const __grid_constant__ Params p) {
+template <int STORE, int ROW_TILES>
+__global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention_quant_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int RG = HALF_ROWS ? 1 : 2;                   // rows a lane has: g, and g + 8
+    constexpr int ROWS = 8 * ROW_TILES;
+    static_assert(ROWS * O_STRIDE * 4 + ROWS * 8 <= WARP_BYTES, "a warp's sums lie over its slots");
     int* const first = reinterpret_cast<int*>(smem + WARPS * WARP_BYTES);     // [segments + 1] the line before each segment
     __shared__ int scan_s[WARPS + 1], ticket_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -147,7 +161,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel
     int before = 0;
     for (int base = 0; base < p.segments; base += THREADS) {
         int mine = 0;
-        if (base + tid < p.segments) { const Segment c = make_segment(p, base + tid); mine = c.row_tiles * p.Hkv * (c.n + PIECE_COST); }
+        if (base + tid < p.segments) { const Segment c = make_segment<ROWS>(p, base + tid); mine = c.row_tiles * p.Hkv * (c.n + PIECE_COST); }
         int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += up; }
@@ -173,33 +187,101 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel
     unsigned char* const mine = smem + warp * WARP_BYTES;
     const uint32_t slots = smem_addr(mine);
     const int page_mask = (1 << p.page_shift) - 1;
+    // Rows of an MMA are keys 4 (r / 2) + r % 2 for r < 8, and two further for r + 8: this lane's key rows are g and g + 8 of a tile of
+    // 16, its values those of keys 4 t .. 4 t + 3.
+    const int key_k = 4 * (g >> 1) + (g & 1), key_v = 4 * t;
+    const uint8_t* const k_lane = p.k_codes + t * KU;
+    const uint8_t* const v_lane = p.v_codes + g * VU;
 
     for (int w = w_begin; w < w_end;) {
         while (first[seg + 1] <= w) ++seg;
-        const Segment c = make_segment(p, seg);
+        const Segment c = make_segment<ROWS>(p, seg);
         const int per = c.n + PIECE_COST, off = w - first[seg], item = off / per, at = off - item * per;
         const int to = min(per, at + w_end - w);
         const int item_first = w - at + PIECE_COST;          // where the row tile's first unit lies in the line
         const int begin = max(0, at - PIECE_COST), end = max(begin, to - PIECE_COST);
         w += to - at;
         if (begin == end) continue;
-        const int hk = item / c.row_tiles, row0 = (item - hk * c.row_tiles) << 4;
-        const int rows = min(16, c.q_len * p.group - row0);
+        const int hk = item / c.row_tiles, row0 = (item - hk * c.row_tiles) * ROWS;
+        const int rows = min(ROWS, c.q_len * p.group - row0);
         const int pos_first = c.start + row0 / p.group, pos_last = c.start + (row0 + rows - 1) / p.group;
         const int lo_first = first_seen_key(pos_first, p.reach), lo_last = first_seen_key(pos_last, p.reach);
         const int* const table = p.block_table + (size_t)seg * p.table_stride;
 
-        // This lane's rows: queries as fragments, brought to about 1 by a power of two that goes into the score's factor.
-        uint32_t qf[KN * KU / 4][2 * RG];
-        float factor[RG], slope[RG];
-        int pos[RG], lo[RG];
+        auto key_of = [&](int i) -> int { return (i < c.n_keep ? i : c.tile_begin - c.n_keep + i) * UNIT + warp * WARP_KEYS; };
+        // The pool's rows of this lane's keys and of its values, of both halves of 32 keys (-1: none that any row sees), one tile
+        // before they are fetched.
+        int row_k[2], row_v[2];
+        auto row_of = [&](int key) -> int {                  // of the four neighbouring keys from `key` on
+            if (key > pos_last || (key + 3 < lo_first && key >= c.keep)) return -1;
+            const int place = key >> p.page_shift;
+            const int page = place < p.table_stride ? __ldg(table + place) : -1;
+            if (page >= 0 && page < p.num_pages) return ((page * p.Hkv + hk) << p.page_shift) + (key & page_mask);
+            atomicOr(p.err, KVB_DEV_BAD_PAGE);
+            return -1;
+        };
+        auto lookup = [&](int i) {
+            if (i >= end) return;
+            const int key0 = key_of(i);
 #pragma unroll
-        for (int r = 0; r < RG; ++r) {
-            const int row = row0 + g + 8 * r, token = row / p.group, head = hk * p.group + row - token * p.group;
-            const bool there = g + 8 * r < rows;
-            pos[r] = there ? c.start + token : 0;
-            lo[r] = first_seen_key(pos[r], p.reach);
-            slope[r] = there && p.slopes ? p.slopes[head] : 0.f;
+            for (int s = 0; s < 2; ++s) {
+                const int key = key0 + 16 * s;
+                if (p.page_shift >= 4 && key + 15 <= pos_last && key >= lo_first) {      // one page, all of it seen by some row
+                    const int row = row_of(key);
+                    row_k[s] = row < 0 ? -1 : row + 4 * (g >> 1);
+                    row_v[s] = row < 0 ? -1 : row + key_v;
+                } else {
+                    row_k[s] = row_of(key + 4 * (g >> 1));
+                    row_v[s] = row_of(key + key_v);
+                }
+            }
+        };
+        auto fetch = [&](int i, int stage) {
+            if (i < end) {
+                const int key0 = key_of(i);
+                const uint32_t base = slots + stage * STAGE_BYTES;
+                const bool all = key0 + WARP_KEYS - 1 <= pos_last && key0 >= lo_first;
+                auto seen = [&](int key) { return all || (key <= pos_last && (key >= lo_first || key < c.keep)); };
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const bool has_k = row_k[s] >= 0, has_v = row_v[s] >= 0;
+                    const int at_k = has_k ? row_k[s] : 0, at_v = has_v ? row_v[s] : 0;
+                    const uint8_t* const from_k = k_lane + (size_t)(at_k + (g & 1)) * D;
+                    const uint8_t* const from_v = v_lane + (size_t)at_v * D;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const bool there = has_k && seen(key0 + 16 * s + key_k + 2 * n);
+#pragma unroll
+                        for (int u = 0; u < KN; ++u)
+                            copy_async<KU>(base + (((s * 2 + n) * KN + u) * 32 + lane) * KU, from_k + 2 * n * D + u * 4 * KU, there);
+                    }
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4) {
+                        const bool there = has_v && seen(key0 + 16 * s + key_v + i4);
+#pragma unroll
+                        for (int u = 0; u < VN; ++u)
+                            copy_async<VU>(base + K_BYTES + (((s * 4 + i4) * VN + u) * 32 + lane) * VU, from_v + i4 * D + u * 8 * VU, there);
+                    }
+                    copy_async<4>(base + K_BYTES + V_BYTES + (2 * s * 32 + lane) * 4, p.k_scales + at_k, has_k);
+                    copy_async<4>(base + K_BYTES + V_BYTES + ((2 * s + 1) * 32 + lane) * 4, p.v_scales + at_k, has_k);
+                }
+            }
+            copies_commit();
+        };
+        lookup(begin);
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) { fetch(begin + s, s); lookup(begin + s + 1); }
+
+        // Queries as fragments, brought to about 1 by a power of two that goes into the score's factor: this lane holds numbers of row
+        // 8 j + g, and the scores of rows 8 j + 2 t and the next.
+        uint32_t qf[ROW_TILES][KN * KU / 4][2];
+        float factor[ROW_TILES][2], slope[ROW_TILES][2];
+        int pos[ROW_TILES][2], lo[ROW_TILES][2];
+        const bool biased = p.cap > 0.f || p.slopes;
+#pragma unroll
+        for (int j = 0; j < ROW_TILES; ++j) {
+            const int row = row0 + 8 * j + g, token = row / p.group, head = hk * p.group + row - token * p.group;
+            const bool there = 8 * j + g < rows;
             uint2 raw[KN * KU / 4];
             uint32_t top = 0u;
             const bf16* const from = p.q + ((size_t)(c.q_start + token) * p.Hq + head) * D + t * KU;
@@ -211,171 +293,136 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int e = top == 0u || top >= 0x7f80u ? 0 : min(100, max(-100, (int)(top >> 7) - 127));
-            const float down = __int_as_float((127 - e) << 23);
-            factor[r] = p.scale * __int_as_float((127 + e) << 23);
+            const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23);
 #pragma unroll
-            for (int k = 0; k < KN * KU / 4; ++k) {
-                qf[k][r] = pack(__uint_as_float(raw[k].x << 16) * down, __uint_as_float(raw[k].x & 0xffff0000u) * down);
-                qf[k][RG + r] = pack(__uint_as_float(raw[k].y << 16) * down, __uint_as_float(raw[k].y & 0xffff0000u) * down);
+            for (int k = 0; k < KN * KU / 4; ++k) {          // the pairs of a word that `halves` makes
+                qf[j][k][0] = pack(__uint_as_float(raw[k].x << 16) * down, __uint_as_float(raw[k].y << 16) * down);
+                qf[j][k][1] = pack(__uint_as_float(raw[k].x & 0xffff0000u) * down, __uint_as_float(raw[k].y & 0xffff0000u) * down);
+            }
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+                const int r = 8 * j + 2 * t + e2, token2 = (row0 + r) / p.group;
+                pos[j][e2] = r < rows ? c.start + token2 : 0;
+                lo[j][e2] = first_seen_key(pos[j][e2], p.reach);
+                slope[j][e2] = r < rows && p.slopes ? p.slopes[hk * p.group + row0 + r - token2 * p.group] : 0.f;
+                factor[j][e2] = p.scale * CODE_SCALE<STORE> * __shfl_sync(0xffffffffu, up, 4 * (2 * t + e2)) * (biased ? 1.f : 1.4426950408889634f);
             }
         }
-        const bool biased = p.cap > 0.f || p.slopes;
-        if (!biased)
-#pragma unroll
-            for (int r = 0; r < RG; ++r) factor[r] *= 1.4426950408889634f;
 
-        auto key_of = [&](int i) -> int { return (i < c.n_keep ? i : c.tile_begin - c.n_keep + i) * UNIT + warp * WARP_KEYS; };
-        // Pages of the four neighbouring keys that hold this lane's key rows and value rows, of both halves of 32 keys.
-        int page_k[2], page_v[2];
-        auto page_of = [&](int key) -> int {
-            if (key > pos_last || (key + 3 < lo_first && key >= c.keep)) return -1;
-            const int place = key >> p.page_shift;
-            const int page = place < p.table_stride ? __ldg(table + place) : -1;
-            if (page >= 0 && page < p.num_pages) return page;
-            atomicOr(p.err, KVB_DEV_BAD_PAGE);
-            return -1;
-        };
-        auto lookup = [&](int i) {
-            if (i >= end) return;
-            const int key0 = key_of(i);
+        float o[ROW_TILES][VN * VU / 2][4];                  // sums of columns (of this lane's) 2 x and 2 x + 1 for its two rows
+        float m[ROW_TILES][2], l[ROW_TILES][2];
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                page_k[s] = page_of(key0 + 16 * s + 4 * (g >> 1));
-                page_v[s] = page_of(key0 + 16 * s + 4 * t);
-            }
-        };
-        auto fetch = [&](int i, int stage) {
-            if (i < end) {
-                const int key0 = key_of(i);
-                const uint32_t base = slots + stage * STAGE_BYTES;
-                auto seen = [&](int key) { return key <= pos_last && (key >= lo_first || key < c.keep); };
+        for (int j = 0; j < ROW_TILES; ++j) {
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const int kk = key0 + 16 * s + 4 * (g >> 1), vv = key0 + 16 * s + 4 * t;
-                    const bool has_k = page_k[s] >= 0, has_v = page_v[s] >= 0;
-                    const size_t row_k = has_k ? ((((size_t)page_k[s] * p.Hkv + hk) << p.page_shift) + (kk & page_mask)) : 0;
-                    const size_t row_v = has_v ? ((((size_t)page_v[s] * p.Hkv + hk) << p.page_shift) + (vv & page_mask)) : 0;
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const int more = 2 * n + (g & 1);
-                        const bool there = has_k && seen(kk + more);
-                        const uint8_t* const from = p.k_codes + (there ? (row_k + more) * D + t * KU : 0);
-#pragma unroll
-                        for (int u = 0; u < KN; ++u)
-                            copy_async<KU>(base + (((s * 2 + n) * KN + u) * 32 + lane) * KU, from + u * 4 * KU, there);
-                    }
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) {
-                        const bool there = has_v && seen(vv + i4);
-                        const uint8_t* const from = p.v_codes + (there ? (row_v + i4) * D + g * VU : 0);
-#pragma unroll
-                        for (int u = 0; u < VN; ++u)
-                            copy_async<VU>(base + K_BYTES + (((s * 4 + i4) * VN + u) * 32 + lane) * VU, from + u * 8 * VU, there);
-                    }
-                    copy_async<4>(base + K_BYTES + V_BYTES + (2 * s * 32 + lane) * 4, p.k_scales + row_v, has_v);
-                    copy_async<4>(base + K_BYTES + V_BYTES + ((2 * s + 1) * 32 + lane) * 4, p.v_scales + row_v, has_v);
-                }
-            }
-            copies_commit();
-        };
-
-        float o[VN * VU][4];
-#pragma unroll
-        for (int i = 0; i < VN * VU; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float m[RG], l[RG];
-#pragma unroll
-        for (int r = 0; r < RG; ++r) { m[r] = NEG_INF; l[r] = 0.f; }
+            for (int i = 0; i < VN * VU / 2; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
+            m[j][0] = m[j][1] = NEG_INF;
+            l[j][0] = l[j][1] = 0.f;
+        }
 
         // 32 keys from `key0` on, whose bytes are there.  MASKED: some row may miss one of them.
         auto tile = [&](int key0, int stage, auto masked_tag) {
             constexpr bool MASKED = decltype(masked_tag)::value;
             const uint32_t base = slots + stage * STAGE_BYTES;
-            float s[2][2][4];
+            float s[2][ROW_TILES][4];                        // [half][eight of rows][key row g or g + 8, query row]
             uint32_t kb[2], vb[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int n = 0; n < 2; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
+                for (int j = 0; j < ROW_TILES; ++j) s[h][j][0] = s[h][j][1] = s[h][j][2] = s[h][j][3] = 0.f;
                 read_slot<4>(base + K_BYTES + V_BYTES + (2 * h * 32 + lane) * 4, &kb[h]);
                 read_slot<4>(base + K_BYTES + V_BYTES + ((2 * h + 1) * 32 + lane) * 4, &vb[h]);
-#pragma unroll
-                for (int u = 0; u < KN; ++u)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        uint32_t word[KU / 4];
-                        read_slot<KU>(base + (((h * 2 + n) * KN + u) * 32 + lane) * KU, word);
-#pragma unroll
-                        for (int k = 0; k < KU / 4; ++k) {
-                            const uint32_t x = flipped<STORE>(word[k]);
-                            mma<HALF_ROWS>(s[h][n], qf[u * (KU / 4) + k], halves<STORE, 0>(x), halves<STORE, 1>(x));
-                        }
-                    }
             }
-            // Exponents of the weights that the value codes get: score (base 2) + the value row's exponent.
-            float top[RG], inv[2][4];
 #pragma unroll
-            for (int r = 0; r < RG; ++r) top[r] = NEG_INF;
-            uint32_t hidden[RG];
+            for (int u = 0; u < KN; ++u)
 #pragma unroll
-            for (int r = 0; r < RG; ++r) hidden[r] = 0u;
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t word[2][KU / 4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                    for (int n = 0; n < 2; ++n) read_slot<KU>(base + (((h * 2 + n) * KN + u) * 32 + lane) * KU, word[n]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int kbyte = (kb[h] >> (8 * i)) & 255, vbyte = (vb[h] >> (8 * i)) & 255;
-                    const float up = __int_as_float(kbyte << 23);
-                    const float shift = __int_as_float(0x4b000000 | vbyte) - 8388735.f;           // vbyte - 127
-                    inv[h][i] = __int_as_float((254 - vbyte) << 23);                              // -infinity for a row that is not finite
-                    const int key = key0 + 16 * h + 4 * t + i;
+                    for (int k = 0; k < KU / 4; ++k) {
+                        uint32_t a[4];
+                        halves<STORE>(word[0][k], a[0], a[2]);
+                        halves<STORE>(word[1][k], a[1], a[3]);
 #pragma unroll
-                    for (int r = 0; r < RG; ++r) {
-                        float x = s[h][i >> 1][(i & 1) + 2 * r] * up * factor[r];
-                        if (biased) {
-                            if (p.cap > 0.f) x = p.cap * (1.f - __fdividef(2.f, 1.f + ex2(x / p.cap * 2.885390081777927f)));
-                            x = (x - slope[r] * (float)(pos[r] - key)) * 1.4426950408889634f;
-                        }
-                        x += shift;
-                        if (MASKED && !(key <= pos[r] && (key >= lo[r] || key < c.keep))) { x = NEG_INF; hidden[r] |= 1u << (4 * h + i); }
-                        s[h][i >> 1][(i & 1) + 2 * r] = x;
-                        top[r] = fmaxf(top[r], x);
+                        for (int j = 0; j < ROW_TILES; ++j) mma(s[h][j], a[0], a[1], a[2], a[3], qf[j][u * (KU / 4) + k]);
                     }
                 }
-            bool moved = false;
-            float base_m[RG], corr[RG];
+            // Exponents of the weights that the value codes get: score (base 2) + the value row's exponent.
+            float top[ROW_TILES][2], inv[2][2];
+            uint32_t hidden = 0u;                            // (MASKED) a bit a score
 #pragma unroll
-            for (int r = 0; r < RG; ++r) {
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                const float now = fmaxf(m[r], top[r]);
-                base_m[r] = now == NEG_INF ? 0.f : now;
-                corr[r] = ex2(m[r] - base_m[r]);
-                moved |= now > m[r];
-                m[r] = now;
-                l[r] *= corr[r];
-            }
+            for (int j = 0; j < ROW_TILES; ++j) top[j][0] = top[j][1] = NEG_INF;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int n = 0; n < 2; ++n) {
+                    const int at_byte = 8 * ((g & 1) + 2 * n);
+                    const int kbyte = (kb[h] >> at_byte) & 255, vbyte = (vb[h] >> at_byte) & 255;
+                    const float up = __int_as_float(kbyte << 23);
+                    const float shift = __int_as_float(0x4b000000 | vbyte) - 8388735.f;           // vbyte - 127
+                    inv[h][n] = __int_as_float((254 - vbyte) << 23);                              // -infinity for a row that is not finite
+                    const int key = key0 + 16 * h + key_k + 2 * n;
 #pragma unroll
-                    for (int r = 0; r < RG; ++r) {
-                        float& x = s[h][i >> 1][(i & 1) + 2 * r];
-                        x = ex2(x - base_m[r]);
-                        l[r] = fmaf(x, MASKED && ((hidden[r] >> (4 * h + i)) & 1u) ? 0.f : inv[h][i], l[r]);
-                    }
+                    for (int j = 0; j < ROW_TILES; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float x = s[h][j][2 * n + e] * up * factor[j][e];
+                            if (biased) {
+                                if (p.cap > 0.f) x = p.cap * (1.f - __fdividef(2.f, 1.f + ex2(x / p.cap * 2.885390081777927f)));
+                                x = (x - slope[j][e] * (float)(pos[j][e] - key)) * 1.4426950408889634f;
+                            }
+                            x += shift;
+                            if (MASKED && !(key <= pos[j][e] && (key >= lo[j][e] || key < c.keep))) {
+                                x = NEG_INF;
+                                hidden |= 1u << (((2 * h + n) * ROW_TILES + j) * 2 + e);
+                            }
+                            s[h][j][2 * n + e] = x;
+                            top[j][e] = fmaxf(top[j][e], x);
+                        }
+                }
+            bool moved = false;
+            float base_m[ROW_TILES][2], corr[ROW_TILES][2];
+#pragma unroll
+            for (int j = 0; j < ROW_TILES; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top[j][e] = fmaxf(top[j][e], __shfl_xor_sync(0xffffffffu, top[j][e], x));
+                    const float now = fmaxf(m[j][e], top[j][e]);
+                    base_m[j][e] = now == NEG_INF ? 0.f : now;
+                    corr[j][e] = ex2(m[j][e] - base_m[j][e]);
+                    moved |= now > m[j][e];
+                    m[j][e] = now;
+                    l[j][e] *= corr[j][e];
+                }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int j = 0; j < ROW_TILES; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float& x = s[h][j][2 * n + e];
+                            x = ex2(x - base_m[j][e]);
+                            l[j][e] = fmaf(x, MASKED && ((hidden >> (((2 * h + n) * ROW_TILES + j) * 2 + e)) & 1u) ? 0.f : inv[h][n], l[j][e]);
+                        }
             if (__any_sync(0xffffffffu, moved)) {            // the maxima seldom move once a few tiles are in
 #pragma unroll
-                for (int i = 0; i < VN * VU; ++i)
+                for (int j = 0; j < ROW_TILES; ++j)
 #pragma unroll
-                    for (int e = 0; e < 2 * RG; ++e) o[i][e] *= corr[e >> 1];
+                    for (int i = 0; i < VN * VU / 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[j][i][e] *= corr[j][e & 1];
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t pa[2 * RG];
+                uint32_t pf[ROW_TILES][2];
 #pragma unroll
-                for (int r = 0; r < RG; ++r) {
-                    pa[r] = pack(s[h][0][2 * r], s[h][0][2 * r + 1]);
-                    pa[RG + r] = pack(s[h][1][2 * r], s[h][1][2 * r + 1]);
+                for (int j = 0; j < ROW_TILES; ++j) {
+                    pf[j][0] = turned(pack(s[h][j][0], s[h][j][1]));
+                    pf[j][1] = turned(pack(s[h][j][2], s[h][j][3]));
                 }
 #pragma unroll
                 for (int u = 0; u < VN; ++u) {
@@ -383,23 +430,19 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel
 #pragma unroll
                     for (int i = 0; i < 4; ++i) read_slot<VU>(base + K_BYTES + (((h * 4 + i) * VN + u) * 32 + lane) * VU, v[i]);
 #pragma unroll
-                    for (int k = 0; k < VU / 4; ++k) {
-                        // Four keys' words, a byte a column: bytes of neighbouring keys side by side.
-                        const uint32_t a_lo = flipped<STORE>(__byte_perm(v[0][k], v[1][k], 0x5140)), a_hi = flipped<STORE>(__byte_perm(v[0][k], v[1][k], 0x7362));
-                        const uint32_t b_lo = flipped<STORE>(__byte_perm(v[2][k], v[3][k], 0x5140)), b_hi = flipped<STORE>(__byte_perm(v[2][k], v[3][k], 0x7362));
-                        float(*const to)[4] = &o[u * VU + 4 * k];
-                        mma<HALF_ROWS>(to[0], pa, halves<STORE, 0>(a_lo), halves<STORE, 0>(b_lo));
-                        mma<HALF_ROWS>(to[1], pa, halves<STORE, 1>(a_lo), halves<STORE, 1>(b_lo));
-                        mma<HALF_ROWS>(to[2], pa, halves<STORE, 0>(a_hi), halves<STORE, 0>(b_hi));
-                        mma<HALF_ROWS>(to[3], pa, halves<STORE, 1>(a_hi), halves<STORE, 1>(b_hi));
-                    }
+                    for (int k = 0; k < VU / 4; ++k)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {        // two columns of four keys
+                            uint32_t a[4];
+                            halves<STORE>(__byte_perm(v[0][k], v[1][k], x ? 0x7632 : 0x5410), a[0], a[1]);
+                            halves<STORE>(__byte_perm(v[2][k], v[3][k], x ? 0x7632 : 0x5410), a[2], a[3]);
+#pragma unroll
+                            for (int j = 0; j < ROW_TILES; ++j) mma(o[j][u * (VU / 2) + 2 * k + x], a[0], a[1], a[2], a[3], pf[j]);
+                        }
                 }
             }
         };
 
-        lookup(begin);
-#pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) { fetch(begin + s, s); lookup(begin + s + 1); }
         int stage = 0;
         for (int i = begin; i < end; ++i) {
             // The slots that the next fetch fills were read by this lane alone, in the turn before.
@@ -418,30 +461,30 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel
         // The warps' sums meet in shared memory, over the slots.
         __syncwarp();
         float* const o_s = reinterpret_cast<float*>(mine);
-        float* const ml_s = o_s + 16 * O_STRIDE;
+        float* const ml_s = o_s + ROWS * O_STRIDE;
 #pragma unroll
-        for (int r = 0; r < RG; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        for (int j = 0; j < ROW_TILES; ++j)
 #pragma unroll
-            for (int u = 0; u < VN; ++u)
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * j + 2 * t + e;
 #pragma unroll
-                for (int b = 0; b < VU; b += 4)
+                for (int x = 4; x < 32; x <<= 1) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], x);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float(*const x)[4] = &o[u * VU + b];
-                        *reinterpret_cast<float4*>(o_s + (g + 8 * r) * O_STRIDE + 8 * VU * u + VU * (2 * t + e) + b) =
-                            make_float4(x[0][2 * r + e], x[1][2 * r + e], x[2][2 * r + e], x[3][2 * r + e]);
+                for (int u = 0; u < VN; ++u)
+#pragma unroll
+                    for (int k = 0; k < VU / 4; ++k) {
+                        const float(*const x)[4] = &o[j][u * (VU / 2) + 2 * k];
+                        *reinterpret_cast<float4*>(o_s + r * O_STRIDE + 8 * VU * u + VU * g + 4 * k) = make_float4(x[0][e], x[0][2 + e], x[1][e], x[1][2 + e]);
                     }
-            if (t == 0) { ml_s[2 * (g + 8 * r)] = m[r]; ml_s[2 * (g + 8 * r) + 1] = l[r]; }
-        }
+                if (g == 0) { ml_s[2 * r] = m[j][e]; ml_s[2 * r + 1] = l[j][e]; }
+            }
         __syncthreads();
         const int block0 = item_first / share, block1 = (item_first + c.n - 1) / share;
         auto place_of = [&](int b) -> size_t { return (size_t)2 * b + (b * share > item_first ? 0 : 1); };
         auto store_row = [&](int r, int col, float4 x, float M, float L) {
             const int row = row0 + r, token = row / p.group, head = hk * p.group + row - token * p.group;
             if (p.sink) L += ex2(p.sink[head] * 1.4426950408889634f - (M == NEG_INF ? 0.f : M));
-            const float k = L > 0.f ? 1.f / L : L == 0.f ? 0.f : __int_as_float(0x7fffffff);
+            const float k = L > 0.f ? CODE_SCALE<STORE> / L : L == 0.f ? 0.f : __int_as_float(0x7fffffff);
             __nv_bfloat162 a = __floats2bfloat162_rn(x.x * k, x.y * k), b = __floats2bfloat162_rn(x.z * k, x.w * k);
             *reinterpret_cast<uint2*>(p.out + ((size_t)(c.q_start + token) * p.Hq + head) * D + col) =
                 make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
@@ -453,7 +496,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel
             float2 ml[WARPS];
 #pragma unroll
             for (int k = 0; k < WARPS; ++k) {
-                ml[k] = *reinterpret_cast<const float2*>(smem + k * WARP_BYTES + (16 * O_STRIDE + 2 * r) * 4);
+                ml[k] = *reinterpret_cast<const float2*>(smem + k * WARP_BYTES + (ROWS * O_STRIDE + 2 * r) * 4);
                 M = fmaxf(M, ml[k].x);
             }
             const float base_m = M == NEG_INF ? 0.f : M;
@@ -468,75 +511,135 @@ __global__ void __launch_bounds__(THREADS, BLOCKS_PER_SM) attention_quant_kernel
                 store_row(r, col, x, M, L);
             } else {
                 const size_t place = place_of(blockIdx.x);
-                *reinterpret_cast<float4*>(p.part_o + (place * 16 + r) * D + col) = x;
-                if (col == 0) *reinterpret_cast<float2*>(p.part_ml + (place * 16 + r) * 2) = make_float2(M, L);
+                *reinterpret_cast<float4*>(p.part_o + (place * ROWS + r) * D + col) = x;
+                if (col == 0) *reinterpret_cast<float2*>(p.part_ml + (place * ROWS + r) * 2) = make_float2(M, L);
             }
         }
         if (block0 != block1) {
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) ticket_s = atomicAdd(p.tickets + block0, 1);
-            __syncthreads();
-            if (ticket_s == block1 - block0) {
-                // All pieces have left their sums: they are added in order, whichever block came last.
-                __threadfence();
-                if (tid == 0) p.tickets[block0] = 0;
-                for (int idx = tid; idx < rows * (D / 4); idx += THREADS) {
-                    const int r = idx / (D / 4), col = (idx - r * (D / 4)) * 4;
+            // Adds what blocks b0 .. b1 (every `step`th) have left, in order: (row, columns, sums, m, l) go to `put`, after all have been read.
+            auto add_up = [&](int b0, int b1, int step, auto put) {
+                float* const ml_all = reinterpret_cast<float*>(smem);        // weights, m and l of up to GROUP pieces
+                const int n = (b1 - b0) / step + 1;
+                for (int idx = tid; idx < rows * n; idx += THREADS) {
+                    const int k = idx / rows, r = idx - k * rows;
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (place_of(b0 + k * step) * ROWS + r) * 2));
+                    ml_all[2 * (r * GROUP + k)] = ml.x;
+                    ml_all[2 * (r * GROUP + k) + 1] = ml.y;
+                }
+                __syncthreads();
+                for (int i0 = 0; i0 < rows * (D / 4); i0 += THREADS) {
+                    const int idx = i0 + tid;
+                    const bool mine_too = idx < rows * (D / 4);
+                    const int r = mine_too ? idx / (D / 4) : 0, col = mine_too ? (idx - r * (D / 4)) * 4 : 0;
                     float M = NEG_INF, L = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int b = block0; b <= block1; ++b) M = fmaxf(M, __ldcg(p.part_ml + (place_of(b) * 16 + r) * 2));
+                    for (int k = 0; k < n; ++k) M = fmaxf(M, ml_all[2 * (r * GROUP + k)]);
                     const float base_m = M == NEG_INF ? 0.f : M;
-#pragma unroll 4
-                    for (int b = block0; b <= block1; ++b) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (place_of(b) * 16 + r) * 2));
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(p.part_o + (place_of(b) * 16 + r) * D + col));
-                        const float f = ex2(ml.x - base_m);
-                        L = fmaf(f, ml.y, L);
-                        x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+#pragma unroll 1
+                    for (int k0 = 0; k0 < n; k0 += 4) {
+                        float4 y[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k0 + k < n) y[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (place_of(b0 + (k0 + k) * step) * ROWS + r) * D + col));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k0 + k < n) {
+                                const float f = ex2(ml_all[2 * (r * GROUP + k0 + k)] - base_m);
+                                L = fmaf(f, ml_all[2 * (r * GROUP + k0 + k) + 1], L);
+                                x.x = fmaf(f, y[k].x, x.x); x.y = fmaf(f, y[k].y, x.y); x.z = fmaf(f, y[k].z, x.z); x.w = fmaf(f, y[k].w, x.w);
+                            }
                     }
-                    store_row(r, col, x, M, L);
+                    if (mine_too) put(r, col, x, M, L);
+                }
+                __syncthreads();
+            };
+            // The last of `of` blocks to raise a ticket, which it sets back.
+            auto last_of = [&](int* ticket, int of) -> bool {
+                __threadfence();
+                __syncthreads();
+                if (tid == 0) {
+                    ticket_s = atomicAdd(ticket, 1);
+                    if (ticket_s == of - 1) *ticket = 0;
+                }
+                __syncthreads();
+                const bool last = ticket_s == of - 1;
+                if (last) __threadfence();
+                return last;
+            };
+            // Pieces are added in groups of GROUP neighbours, the groups' sums (which lie where their first pieces' lay) in groups again.
+            bool last = true;
+            int step = 1;
+            for (; last && (block1 - block0) / step >= GROUP; step *= GROUP) {
+                const int b0 = block0 + ((int)blockIdx.x - block0) / (step * GROUP) * (step * GROUP);
+                const int members = min(GROUP, (block1 - b0) / step + 1);
+                // A block leads a group of one item that starts in it and of one that goes through it, of each size.
+                last = last_of(p.tickets + ((size_t)(step == 1 ? 0 : step == GROUP ? 1 : 2) * gridDim.x + b0) * 2 + (b0 == block0), members);
+                if (last) {
+                    float* const to_o = p.part_o + place_of(b0) * ROWS * D;
+                    float* const to_ml = p.part_ml + place_of(b0) * ROWS * 2;
+                    add_up(b0, b0 + (members - 1) * step, step, [&](int r, int col, float4 x, float M, float L) {
+                        *reinterpret_cast<float4*>(to_o + r * D + col) = x;
+                        if (col == 0) *reinterpret_cast<float2*>(to_ml + r * 2) = make_float2(M, L);
+                    });
                 }
             }
+            if (last && last_of(p.tickets + (size_t)6 * gridDim.x + block0, (block1 - block0) / step + 1))
+                add_up(block0, block0 + (block1 - block0) / step * step, step, store_row);
         }
         __syncthreads();                                     // the slots are the next piece's
     }
 }
 
-template <int STORE, bool HALF_ROWS>
-static int launch(const Params& p, int blocks, cudaStream_t stream) {
+template <int STORE, int ROW_TILES>
+static int launch(Params p, int sms, long long pieces, cudaStream_t stream) {
     const size_t smem = WARPS * WARP_BYTES + (size_t)(p.segments + 1) * 4;
     static int configured = -1;                              // the device that has been told of the shared memory
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
     if (configured != device) {
-        e = cudaFuncSetAttribute(attention_quant_kernel<STORE, HALF_ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        e = cudaFuncSetAttribute(attention_quant_kernel<STORE, ROW_TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  WARPS * WARP_BYTES + (MAX_SEGMENTS + 1) * 4);
         if (e != cudaSuccess) return (int)e;
         configured = device;
     }
-    kvb_launch(attention_quant_kernel<STORE, HALF_ROWS>, dim3(blocks), dim3(THREADS), smem, stream, p);
+    const int blocks = (int)min((long long)sms * blocks_per_sm<ROW_TILES>(), pieces);
+    p.part_ml = p.part_o + (size_t)2 * blocks * 8 * ROW_TILES * D;
+    kvb_launch(attention_quant_kernel<STORE, ROW_TILES>, dim3(blocks), dim3(THREADS), smem, stream, p);
     return kvb_launch_status();
+}
+
+constexpr int MOST_BLOCKS = 4;         // of any of the kernels, on an SM
+constexpr int MOST_TILES = D <= 64 ? 4 : 2;       // eights of rows at once: what a thread's registers hold
+
+template <int STORE>
+static int launch_rows(const Params& p, long long rows, int sms, long long pieces, cudaStream_t stream) {
+    if (rows <= 8) return launch<STORE, 1>(p, sms, pieces, stream);
+    if (rows <= 16 || MOST_TILES == 2) return launch<STORE, 2>(p, sms, pieces, stream);
+    return launch<STORE, MOST_TILES>(p, sms, pieces, stream);
 }
 
 }  // namespace aq
 
-// How many blocks fill an SM, and segments a launch takes.
-KVB_API int kvb_attention_quant_blocks() { return aq::BLOCKS_PER_SM; }
-KVB_API int kvb_attention_quant_max_segments() { return aq::MAX_SEGMENTS; }
+// What a launch needs for every SM: tickets, and floats of scratch.
+KVB_API int kvb_attention_quant_tickets() { return 7 * aq::MOST_BLOCKS; }
+KVB_API int kvb_attention_quant_scratch() {
+    using namespace aq;
+    const int one = blocks_per_sm<1>() * 8, two = blocks_per_sm<2>() * 16, most = blocks_per_sm<MOST_TILES>() * 8 * MOST_TILES;
+    return 2 * (one > two ? (one > most ? one : most) : two > most ? two : most) * (D + 2);
+}
 
-// Segments of up to `max_q` tokens (the others' rows stay as they are).  page_size: a power of two from 4 on.  scratch:
-// 2 * blocks * 16 * (D + 2) floats; tickets: blocks ints, zero before the first launch (the kernel leaves them zero).
+// Segments of up to `max_q` tokens (the others' rows stay as they are).  page_size: a power of two from 4 on.  scratch and tickets:
+// as above for each of `sms` SMs; the tickets zero before the first launch (the kernel leaves them zero).
 KVB_API int kvb_attention_quant(int store, const void* q, void* out, const void* k_codes, const void* v_codes, const void* k_scales, const void* v_scales,
                                 int num_pages, const int* block_table, int table_stride, int segments, int T, const int* seg_q_start,
                                 const int* seg_q_len, const int* seg_kv_len, int max_q, int Hq, int Hkv, int page_size, int reach, int keep,
-                                const float* sink, const float* slopes, float cap, float scale, float* scratch, int* tickets, int blocks, int min_units,
+                                const float* sink, const float* slopes, float cap, float scale, float* scratch, int* tickets, int sms, int min_units,
                                 int* err, cudaStream_t stream) {
     using namespace aq;
     if (segments <= 0 || T <= 0) return KVB_OK;
     if (store != KVB_E4M3 && store != KVB_INT8) return KVB_ERR_DTYPE;
-    if (Hkv < 1 || Hq % Hkv != 0 || page_size < 4 || (page_size & (page_size - 1)) != 0 || num_pages < 1 || max_q < 1 || keep < 0 || cap < 0.f || blocks < 1 ||
+    if (Hkv < 1 || Hq % Hkv != 0 || page_size < 4 || (page_size & (page_size - 1)) != 0 || num_pages < 1 || max_q < 1 || keep < 0 || cap < 0.f || sms < 1 ||
         min_units < 1 || table_stride < 1)
         return KVB_ERR_SHAPE;
     if (segments > MAX_SEGMENTS) return KVB_ERR_LIMIT;
@@ -544,13 +647,15 @@ KVB_API int kvb_attention_quant(int store, const void* q, void* out, const void*
     if (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3) return KVB_ERR_ALIGN;
     const int group = Hq / Hkv;
     // The line of units is counted in 32 bits.
-    const long long tiles = ((long long)T * group) / 16 + segments, units = (long long)table_stride * page_size / UNIT + 3 + PIECE_COST;
+    const long long tiles = ((long long)T * group) / 8 + segments, units = (long long)table_stride * page_size / UNIT + 3 + PIECE_COST;
     if (tiles * Hkv * units > 0x3fffffffll || (long long)table_stride * page_size > 0x3fffffffll) return KVB_ERR_LIMIT;
+    if ((long long)num_pages * Hkv * page_size > 0x7fffffffll) return KVB_ERR_LIMIT;      // rows of a pool, too
     Params p = {(const bf16*)q, (bf16*)out, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scales, (const uint8_t*)v_scales, num_pages,
                 block_table, table_stride, 0, segments, seg_q_start, seg_q_len, seg_kv_len, max_q, Hq, Hkv, group, reach, keep, scale, cap, sink, slopes,
-                scratch, scratch + (size_t)2 * blocks * 16 * D, tickets, min_units, err};
+                scratch, nullptr, tickets, min_units, err};
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    const bool half_rows = (long long)max_q * group <= 8;
-    if (store == KVB_E4M3) return half_rows ? launch<KVB_E4M3, true>(p, blocks, stream) : launch<KVB_E4M3, false>(p, blocks, stream);
-    return half_rows ? launch<KVB_INT8, true>(p, blocks, stream) : launch<KVB_INT8, false>(p, blocks, stream);
+    // Eights of rows a block takes at once: as many as the longest segment has, as far as registers go.
+    const long long most_rows = (long long)max_q * group;
+    if (store == KVB_E4M3) return launch_rows<KVB_E4M3>(p, most_rows, sms, tiles * Hkv * units, stream);
+    return launch_rows<KVB_INT8>(p, most_rows, sms, tiles * Hkv * units, stream);
 }

@@ -265,8 +265,8 @@ _SIGNATURES = {
                               _c_int, _c_void_p, _c_float, _c_int, _c_void_p],
     },
     "attention_quant": {
-        "kvb_attention_quant_blocks": [],
-        "kvb_attention_quant_max_segments": [],
+        "kvb_attention_quant_tickets": [],
+        "kvb_attention_quant_scratch": [],
         "kvb_attention_quant": [_c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int,
                                 _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_float,
                                 _c_float, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p],
@@ -348,6 +348,7 @@ class CudaKernels(KernelSet):
             raise KernelError(f"kernels are built for sm_100a; device {self.device} is sm_{major}{minor}")
         if bf16_gemm not in ("auto", "tcgen05", "cublas", "simt"):
             raise KernelError(f"unknown bf16_gemm '{bf16_gemm}'")
+        self._device_index = torch.cuda.current_device() if self.device.index is None else self.device.index
         self.bf16_gemm = bf16_gemm
         self._elementwise = _Library("elementwise")
         self._rope = _Library("rope_append")
@@ -355,7 +356,7 @@ class CudaKernels(KernelSet):
         self._gemm_simt = _Library("gemm_simt")
         self._cache_quant = _Library("cache_quant")
         self._expand_cache_planners: Dict[tuple, "CacheExpandPlanner"] = {}
-        self._attn_quant: Dict[int, Tuple[_Library, int]] = {}
+        self._attn_quant: Dict[int, Tuple[_Library, int, int]] = {}
         self._latent = _Library("latent")
         self._recurrent = _Library("recurrent")
         self._scan_wide = _Library("scan_wide")
@@ -449,13 +450,13 @@ class CudaKernels(KernelSet):
     def _stream(self) -> int:
         if self._pinned_stream is not None:
             return self._pinned_stream
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self._device_index)      # 0.1 us, an object for the stream 1.5 us
 
     @contextlib.contextmanager
     def on_current_stream(self):
         """Within the block every launch goes to the stream that is current now (asked for once, not per launch)."""
         saved = self._pinned_stream
-        self._pinned_stream = torch.cuda.current_stream(self.device).cuda_stream
+        self._pinned_stream = torch._C._cuda_getCurrentRawStream(self._device_index)
         try:
             yield
         finally:
@@ -892,18 +893,17 @@ class CudaKernels(KernelSet):
 
     def _quantised_entry(self, kv: PagedKVView, what: str) -> int:
         """The store's code, after the checks of a view of such an entry."""
-        spec = kv.spec
+        spec, k, v, ks, vs = kv.spec, kv.k_pages, kv.v_pages, kv.k_scales, kv.v_scales
         dtype = STORE_DTYPES.get(spec.store)
         if dtype is None:
             raise KernelError(f"{what}: a cache is held as one of {', '.join(STORE_DTYPES)}, not '{spec.store}'")
+        shape = k.shape
         if spec.v_head_dim != spec.head_dim:
             raise KernelError(f"{what}: a cache in eight bits has values as wide as keys")
-        shape = (kv.k_pages.shape[0], spec.num_kv_heads, kv.page_size)
-        if kv.k_pages.dtype != dtype or kv.v_pages.dtype != dtype or kv.k_pages.shape != (*shape, spec.head_dim) or kv.v_pages.shape != kv.k_pages.shape:
+        if k.dtype != dtype or v.dtype != dtype or shape[1:] != (spec.num_kv_heads, kv.page_size, spec.head_dim) or v.shape != shape:
             raise KernelError(f"{what}: pages of a cache held as {spec.store} are {dtype} [pages, kv heads, page size, head size]")
-        for scales in (kv.k_scales, kv.v_scales):
-            if scales is None or scales.dtype != torch.uint8 or scales.shape != shape:
-                raise KernelError(f"{what}: a cache in eight bits has scale bytes, uint8 [pages, kv heads, page size]")
+        if ks is None or vs is None or ks.dtype != torch.uint8 or vs.dtype != torch.uint8 or ks.shape != shape[:3] or vs.shape != shape[:3]:
+            raise KernelError(f"{what}: a cache in eight bits has scale bytes, uint8 [pages, kv heads, page size]")
         return self._STORE_CODES[spec.store]
 
     def _append_quantised(self, qkv, bias, cos, sin, batch: StepBatch, kv: PagedKVView, q_out, num_heads: int, q_norm, k_norm, norm_eps: float,
@@ -978,11 +978,13 @@ class CudaKernels(KernelSet):
     quant_expand_min_rows = 64           # portions of at least this many tokens have their keys and values read back first
     quant_min_units = 2                  # units of 128 keys a block of csrc/attention_quant.cu takes at least
 
-    def _quant_library(self, head_dim: int) -> Tuple[_Library, int]:
+    def _quant_library(self, head_dim: int) -> Tuple[_Library, int, int]:
+        """(the kernels, floats of scratch, tickets)"""
         found = self._attn_quant.get(head_dim)
         if found is None:
             lib = _Library("attention_quant", f"d{head_dim}", [f"-DKVB_HEAD_DIM={head_dim}"])
-            found = self._attn_quant[head_dim] = (lib, int(lib.kvb_attention_quant_blocks()))
+            found = self._attn_quant[head_dim] = (lib, self.sm_count * int(lib.kvb_attention_quant_scratch()),
+                                                  self.sm_count * int(lib.kvb_attention_quant_tickets()))
         return found
 
     def _quantised_attention(self, q, batch: StepBatch, kv: PagedKVView, out, num_heads: int, scale: float, workspace, sink, score_cap, slopes,
@@ -998,40 +1000,36 @@ class CudaKernels(KernelSet):
         group = num_heads // Hkv
         # Codes read in place: bfloat16, four sizes of heads, pages of at least the four keys whose scale bytes are fetched together.
         direct = (q.dtype == torch.bfloat16 and D in (32, 64, 96, 128) and kv.page_size >= 4 and workspace is not None
-                  and S <= self.QUANT_MAX_SEGMENTS and (q.data_ptr() | out.data_ptr() | kv.k_pages.data_ptr() | kv.v_pages.data_ptr()) % 16 == 0
+                  and S <= self.QUANT_MAX_SEGMENTS and kv.k_scales.numel() < 1 << 31 and (q.data_ptr() | out.data_ptr() | kv.k_pages.data_ptr() | kv.v_pages.data_ptr()) % 16 == 0
                   and (kv.k_scales.data_ptr() | kv.v_scales.data_ptr()) % 4 == 0)
         # Read back first: portions of enough rows, and what the codes' own kernel does not take.
-        plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
-        paged = batch.plans.get(PagedAttentionPlanner.name)
-        singles = S if batch.max_q_len == 1 else S if paged is None else paged.counts["decode_items"]
-        expand = (plan is not None and plan.counts["blocks"] > 0 and paged is not None and workspace is not None
-                  and 4 * plan.counts["blocks"] * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES)
-        if direct:
-            # Segments of single tokens keep to their codes; the portions' kernels have to leave them out.
-            expand = expand and batch.max_q_len >= self.quant_expand_min_rows and D % 16 == 0 and group <= 16
-        else:
-            expand = expand and (with_singles or singles == 0)
+        expand = False
+        if not direct or (batch.max_q_len >= self.quant_expand_min_rows and group <= 16):
+            plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
+            paged = batch.plans.get(PagedAttentionPlanner.name)
+            singles = S if batch.max_q_len == 1 or paged is None else paged.counts["decode_items"]
+            expand = (plan is not None and plan.counts["blocks"] > 0 and paged is not None and workspace is not None
+                      and 4 * plan.counts["blocks"] * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES
+                      and (direct or with_singles or singles == 0))
         if expand:
             view = self.expand_cache(batch, kv, q.dtype, workspace, reach)
             portions = batch
-            if direct and singles:
+            if direct and singles:           # single tokens keep to their codes: the portions' kernels leave them out
                 portions = dataclasses.replace(batch, plans={**batch.plans, PagedAttentionPlanner.name: StepPlan(
                     paged.arrays, {**paged.counts, "decode_items": 0})})
             self.paged_attention(q, portions, view, out, num_heads, scale, workspace, sink=sink, score_cap=score_cap, slopes=slopes, reach=reach)
             if not direct or not singles:
                 return
         if direct:
-            lib, per_sm = self._quant_library(D)
-            most = 1 if expand else batch.max_q_len
-            blocks = min(per_sm * self.sm_count, S * Hkv * -(-most * group // 16) * (kv.block_table.shape[1] * kv.page_size // 128 + 3))
-            scratch = workspace.buffer("attn.quant_scratch", (2 * per_sm * self.sm_count * 16 * (D + 2),), torch.float32)
-            tickets = workspace.zeros("attn.quant_tickets", (per_sm * self.sm_count,), torch.int32)
+            lib, floats, tickets_wanted = self._quant_library(D)
+            scratch = workspace.buffer("attn.quant_scratch", (floats,), torch.float32)
+            tickets = workspace.zeros("attn.quant_tickets", (tickets_wanted,), torch.int32)
             self._count("attention_quant")
             _check(lib.kvb_attention_quant(
                 store, _ptr(q), _ptr(out), _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
-                _ptr(kv.block_table), kv.block_table.shape[1], S, T, _ptr(batch.seg_q_start), _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len), most,
-                num_heads, Hkv, kv.page_size, reach, spec.keep_first, _ptr(sink), _ptr(slopes), float(score_cap or 0.0), float(scale),
-                _ptr(scratch), _ptr(tickets), blocks, self.quant_min_units, _ptr(self.error_word), self._stream()), "paged_attention")
+                _ptr(kv.block_table), kv.block_table.shape[1], S, T, _ptr(batch.seg_q_start), _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len),
+                1 if expand else batch.max_q_len, num_heads, Hkv, kv.page_size, reach, spec.keep_first, _ptr(sink), _ptr(slopes), float(score_cap or 0.0), float(scale),
+                _ptr(scratch), _ptr(tickets), self.sm_count, self.quant_min_units, _ptr(self.error_word), self._stream()), "paged_attention")
             return
         self._count("attention_quant_any")
         _check(self._cache_quant.kvb_attention_quant_any(
