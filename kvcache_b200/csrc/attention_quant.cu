@@ -6,21 +6,22 @@
 //   score_j = scale 2^(e_j) (q . c_j),   out = sum_j w_j 2^(f_j) d_j / sum_j w_j,   w_j = 2^(score_j log2 e)
 // with (c, e) a key's and (d, f) a value's row.  The weights that meet the value codes are n_j = 2^(score_j log2 e + f_j - m), m the
 // largest of those exponents so far: at most 1, and what matters for the sum is near 1 whatever the rows' scales are, so that half
-// precision holds them to 2^-11.  The denominator takes n_j 2^(-f_j), in float32.  Codes are exact in half precision, and so
-// are queries once a power of two has brought their row to about 1: products run on mma.sync m16n8k16 (half, float32 sums).
+// precision holds them to 2^-11.  The denominator takes n_j 2^(-f_j), in float32.  Scores are products of codes as they are stored
+// (mma.sync m16n8k32, a step of which takes half the time of one over half precision) by queries in two parts of eight bits; value codes,
+// exact in half precision, meet the weights on mma.sync m16n8k16.
 //
 // Codes are the operand with 16 rows, S^T = K Q^T and O^T = V^T P^T, so that eight query rows - the heads that share a key head,
 // times the tokens of a short portion - fill an MMA, and what a code costs on its way to half precision is paid once for up to
 // ROW_TILES eights of rows.  (Queries as the 16 rows: twice the MMAs and sums in registers for seven heads.)
-// A warp takes 32 keys at a time and needs nothing from any other until its run ends.  The order of an MMA's inner index, and of its
+// A warp takes 32 keys at a time - a block's four in turn - and needs nothing from any other until the block's run ends.  The order of an MMA's inner index, and of its
 // rows, is free as long as all agree, so a lane's share of a tile is bytes that lie together: for the scores 16 (or 8) of a key's
 // numbers, for the sum the same of four neighbouring keys' values.  Each lane copies those bytes itself (cp.async, into slots of
-// shared memory that no other lane touches), a tile ahead, and turns them into half precision in registers: no barrier, no
+// shared memory that no other lane touches), two tiles ahead, and turns them into half precision in registers: no barrier, no
 // bank conflict and no wait for another lane stands in the stream.
 //
-// Work is shared out by keys: units of 128 keys of every (segment, key head, tile of rows), laid end to end, are cut into equal
+// Work is shared out by keys: units of 32 keys of every (segment, key head, tile of rows), laid end to end, are cut into equal
 // runs, one a block, whatever the lengths.  Where a cut divides a row tile's keys, the pieces' sums meet in scratch, two places a
-// block: the last of eight neighbours to finish adds them in order, and so on up to the whole: the same bits whichever is last, and
+// block: the last of sixteen neighbours to finish adds them in order, and so on until 32 are left for the last: the same bits whichever is last, and
 // none of many pieces waits for one block to read them all (131,072 keys of 4 heads in 103 pieces each: 74 us with one
 // block adding all).
 #include "cache_quant.cuh"
@@ -36,7 +37,7 @@ using namespace cq;
 constexpr int D = KVB_HEAD_DIM;
 static_assert(D == 32 || D == 64 || D == 96 || D == 128, "head sizes 32, 64, 96 and 128");
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
-constexpr int WARP_KEYS = 32, UNIT = WARPS * WARP_KEYS;
+constexpr int UNIT = 32;                // keys a warp takes at a time
 constexpr int KU = D % 64 == 0 ? 16 : 8, KN = D / (4 * KU);                       // bytes a copy, copies a key row and lane: four lanes share a key row
 constexpr int VU = D % 128 == 0 ? 16 : D % 64 == 0 ? 8 : 4, VN = D / (8 * VU);    // ... eight lanes share a value row
 constexpr int K_BYTES = 4 * KN * KU * 32, V_BYTES = 8 * VN * VU * 32, STAGE_BYTES = K_BYTES + V_BYTES + 4 * 32 * 4;
@@ -46,9 +47,10 @@ constexpr int O_STRIDE = D + 4;
 // Blocks an SM holds of the kernel for ROW_TILES eights of rows: registers allow 3 of 168 a thread, or 4 of 128, or 2 of 255.
 template <int ROW_TILES> constexpr int blocks_per_sm() { return ROW_TILES == 1 ? (D <= 64 ? 4 : 3) : ROW_TILES == 2 ? (D <= 64 ? 3 : 2) : 2; }
 constexpr int MAX_SEGMENTS = 4096;
-constexpr int GROUP = 8;               // pieces whose sums one block adds up
-constexpr int PIECE_COST = 1;          // what a piece costs beside its keys, in units
+constexpr int GROUP = 16, MOST = 32;   // pieces whose sums one block adds up: of a group, and of the last ones that are left
+constexpr int PIECE_COST = 4;          // what a piece costs beside its keys, in units
 constexpr float NEG_INF = -INFINITY;
+constexpr float HEADROOM = 8.f;
 
 struct Params {
     const bf16* q;             // [T, Hq * D]
@@ -98,6 +100,41 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
+// The same for 32 numbers a row in eight bits: codes as they are stored, by queries split in two parts of eight bits.
+template <int STORE>
+__device__ __forceinline__ void mma8(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
+    if (STORE == KVB_E4M3)
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
+    else
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
+}
+// Two query numbers (their row's largest lies in 1 .. 2) as two codes of the cache's type each, in the lower two bytes; `joined` is the
+// score from their sums.  e4m3: 128 x = high + low / 32, each with four significant bits - all eight of a bfloat16, and what lies 2^-20
+// below the row's largest vanishes.  int8: 16320 x = 256 high + low, off by 2^-15 of the row's largest at most.  Either is far below what
+// rounds the weights (2^-11).
+template <int STORE>
+__device__ __forceinline__ void split_queries(float x0, float x1, uint32_t& high, uint32_t& low) {
+    if (STORE == KVB_E4M3) {
+        const float2 y = make_float2(128.f * x0, 128.f * x1);
+        const __nv_fp8x2_storage_t h = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+        const float2 z = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(h, __NV_E4M3)));
+        high = h;
+        low = __nv_cvt_float2_to_fp8x2(make_float2(32.f * (y.x - z.x), 32.f * (y.y - z.y)), __NV_SATFINITE, __NV_E4M3);
+    } else {
+        const int y0 = __float2int_rn(16320.f * x0), y1 = __float2int_rn(16320.f * x1);      // |y| < 127.5 * 256
+        const int h0 = (y0 + 128) >> 8, h1 = (y1 + 128) >> 8;
+        high = __byte_perm((uint32_t)h0, (uint32_t)h1, 0x0040) & 0xffffu;
+        low = __byte_perm((uint32_t)(y0 - 256 * h0), (uint32_t)(y1 - 256 * h1), 0x0040) & 0xffffu;
+    }
+}
+template <int STORE>
+__device__ __forceinline__ float joined(uint32_t high, uint32_t low) {
+    if (STORE == KVB_E4M3) return fmaf(__uint_as_float(low), 1.f / 32.f, __uint_as_float(high));
+    return (float)(256 * (int)high + (int)low);
+}
+template <int STORE> constexpr float QUERY_SCALE = STORE == KVB_E4M3 ? 1.f / 128.f : 1.f / 16320.f;
 // The 8 x 8 matrix of 16-bit numbers that a warp holds, a row a group of four lanes, turned.
 __device__ __forceinline__ uint32_t turned(uint32_t x) {
     uint32_t y;
@@ -154,34 +191,45 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
     constexpr int ROWS = 8 * ROW_TILES;
     static_assert(ROWS * O_STRIDE * 4 + ROWS * 8 <= WARP_BYTES, "a warp's sums lie over its slots");
     int* const first = reinterpret_cast<int*>(smem + WARPS * WARP_BYTES);     // [segments + 1] the line before each segment
-    __shared__ int scan_s[WARPS + 1], ticket_s;
+    __shared__ int ticket_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-    // The step's lengths are metadata that no kernel before this one writes.
-    int before = 0;
-    for (int base = 0; base < p.segments; base += THREADS) {
-        int mine = 0;
-        if (base + tid < p.segments) { const Segment c = make_segment<ROWS>(p, base + tid); mine = c.row_tiles * p.Hkv * (c.n + PIECE_COST); }
-        int sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += up; }
-        if (lane == 31) scan_s[warp] = sum;
-        __syncthreads();
-        int below = before, all = before;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) { if (w < warp) below += scan_s[w]; all += scan_s[w]; }
-        if (base + tid < p.segments) first[base + tid] = below + sum - mine;
-        before = all;
-        __syncthreads();
+    // Few row tiles: each is cut into equal pieces of at least `share` units, a block a piece, so that none waits for a second.  `share` is
+    // such that the pieces are no more than the blocks.  Many: the line of all units, with what a piece costs beside them, is cut into equal runs.
+    // first[s]: the pieces, or the line, before segment s.  The step's lengths are metadata that no kernel before this one writes.
+    const int blocks = (int)gridDim.x;
+    int units = 0, items = 0;
+    for (int s = lane; s < p.segments; s += 32) {
+        const Segment c = make_segment<ROWS>(p, s);
+        items += c.row_tiles * p.Hkv;
+        units += c.row_tiles * p.Hkv * c.n;
     }
-    if (tid == 0) first[p.segments] = before;
+    units = __reduce_add_sync(0xffffffffu, units);
+    items = __reduce_add_sync(0xffffffffu, items);
+    const bool whole = items * 8 <= blocks;
+    const int total = units + items * PIECE_COST;
+    const int share = max(p.min_units, whole ? (units + blocks - items - 1) / max(1, blocks - items) : (total + blocks - 1) / blocks);
+    if (warp == 0) {
+        int before = 0;
+        for (int base = 0; base < p.segments; base += 32) {
+            int sum = 0, mine = 0;
+            if (base + lane < p.segments) {
+                const Segment c = make_segment<ROWS>(p, base + lane);
+                mine = sum = c.row_tiles * p.Hkv * (whole ? (c.n + share - 1) / share : c.n + PIECE_COST);
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += up; }
+            if (base + lane < p.segments) first[base + lane] = before + sum - mine;
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) first[p.segments] = before;
+    }
     __syncthreads();
-    const int total = before;
-    const int share = max(p.min_units, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-    const int w_begin = (int)min((long long)total, (long long)blockIdx.x * share), w_end = min(total, w_begin + share);
+    const int line = first[p.segments];
+    const int w_begin = (int)min((long long)line, whole ? (long long)blockIdx.x : (long long)blockIdx.x * share), w_end = min(line, w_begin + (whole ? 1 : share));
     int seg = 0;
     for (int hi = p.segments; hi - seg > 1;) { const int mid = (seg + hi) >> 1; if (first[mid] <= w_begin) seg = mid; else hi = mid; }
-    pdl_wait();
+    pdl_wait();                                              // blocks without work as well: what comes next may count on all before it
     pdl_launch_dependents();
 
     unsigned char* const mine = smem + warp * WARP_BYTES;
@@ -190,17 +238,35 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
     // Rows of an MMA are keys 4 (r / 2) + r % 2 for r < 8, and two further for r + 8: this lane's key rows are g and g + 8 of a tile of
     // 16, its values those of keys 4 t .. 4 t + 3.
     const int key_k = 4 * (g >> 1) + (g & 1), key_v = 4 * t;
+    // Selectors that put the scale byte of key row g, or g + 8, of four neighbours' into a word's highest byte.
+    const uint32_t pick_first = g & 1 ? 0x1444u : 0x0444u, pick_second = g & 1 ? 0x3444u : 0x2444u;
     const uint8_t* const k_lane = p.k_codes + t * KU;
     const uint8_t* const v_lane = p.v_codes + g * VU;
 
     for (int w = w_begin; w < w_end;) {
         while (first[seg + 1] <= w) ++seg;
         const Segment c = make_segment<ROWS>(p, seg);
-        const int per = c.n + PIECE_COST, off = w - first[seg], item = off / per, at = off - item * per;
-        const int to = min(per, at + w_end - w);
-        const int item_first = w - at + PIECE_COST;          // where the row tile's first unit lies in the line
-        const int begin = max(0, at - PIECE_COST), end = max(begin, to - PIECE_COST);
-        w += to - at;
+        const int off = w - first[seg];
+        int item, begin, end, block0, block1;                // a row tile, units of its list, and the blocks that have some of them
+        if (whole) {
+            const int pieces = (c.n + share - 1) / share, size = (c.n + pieces - 1) / pieces;
+            item = off / pieces;
+            begin = min(c.n, (off - item * pieces) * size);
+            end = min(c.n, begin + size);
+            block0 = w - (off - item * pieces);
+            block1 = block0 + (c.n + size - 1) / size - 1;
+            ++w;
+        } else {
+            const int per = c.n + PIECE_COST;
+            item = off / per;
+            const int at = off - item * per, to = min(per, at + w_end - w);
+            const int item_first = w - at + PIECE_COST;      // where the row tile's first unit lies in the line
+            begin = max(0, at - PIECE_COST);
+            end = max(begin, to - PIECE_COST);
+            block0 = item_first / share;
+            block1 = (item_first + c.n - 1) / share;
+            w += to - at;
+        }
         if (begin == end) continue;
         const int hk = item / c.row_tiles, row0 = (item - hk * c.row_tiles) * ROWS;
         const int rows = min(ROWS, c.q_len * p.group - row0);
@@ -208,96 +274,128 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         const int lo_first = first_seen_key(pos_first, p.reach), lo_last = first_seen_key(pos_last, p.reach);
         const int* const table = p.block_table + (size_t)seg * p.table_stride;
 
-        auto key_of = [&](int i) -> int { return (i < c.n_keep ? i : c.tile_begin - c.n_keep + i) * UNIT + warp * WARP_KEYS; };
-        // The pool's rows of this lane's keys and of its values, of both halves of 32 keys (-1: none that any row sees), one tile
-        // before they are fetched.
-        int row_k[2], row_v[2];
-        auto row_of = [&](int key) -> int {                  // of the four neighbouring keys from `key` on
-            if (key > pos_last || (key + 3 < lo_first && key >= c.keep)) return -1;
+        auto key_of = [&](int i) -> int { return (i < c.n_keep ? i : c.tile_begin - c.n_keep + i) * UNIT; };
+        // Pages of this lane's four neighbouring key rows and of its four values, of both halves of 32 keys, asked for one tile before
+        // they are looked at; -1: none that any row sees.
+        struct Pages { int k[2], v[2]; };
+        auto page_of = [&](int key) -> int {                 // of the four neighbouring keys from `key` on
             const int place = key >> p.page_shift;
-            const int page = place < p.table_stride ? __ldg(table + place) : -1;
-            if (page >= 0 && page < p.num_pages) return ((page * p.Hkv + hk) << p.page_shift) + (key & page_mask);
-            atomicOr(p.err, KVB_DEV_BAD_PAGE);
-            return -1;
+            return key > pos_last || (key + 3 < lo_first && key >= c.keep) || place >= p.table_stride ? -1 : __ldg(table + place);
         };
-        auto lookup = [&](int i) {
-            if (i >= end) return;
-            const int key0 = key_of(i);
+        auto lookup = [&](int i) -> Pages {
+            Pages x = {{-1, -1}, {-1, -1}};
+            if (i < end) {
+                const int key0 = key_of(i);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int key = key0 + 16 * s;
-                if (p.page_shift >= 4 && key + 15 <= pos_last && key >= lo_first) {      // one page, all of it seen by some row
-                    const int row = row_of(key);
-                    row_k[s] = row < 0 ? -1 : row + 4 * (g >> 1);
-                    row_v[s] = row < 0 ? -1 : row + key_v;
-                } else {
-                    row_k[s] = row_of(key + 4 * (g >> 1));
-                    row_v[s] = row_of(key + key_v);
+                for (int s = 0; s < 2; ++s) {
+                    x.k[s] = page_of(key0 + 16 * s + 4 * (g >> 1));
+                    x.v[s] = p.page_shift >= 4 && key0 + 16 * s + 15 <= pos_last && key0 + 16 * s >= lo_first ? x.k[s] : page_of(key0 + 16 * s + key_v);
                 }
             }
+            return x;
         };
-        auto fetch = [&](int i, int stage) {
+        // The pool's row of `key`, which lies in `page`; -1 without one, which is reported if some row sees the key.
+        auto row_of = [&](int page, int key) -> int {
+            if (page >= 0 && page < p.num_pages) return ((page * p.Hkv + hk) << p.page_shift) + (key & page_mask);
+            if (key <= pos_last && (key + 3 >= lo_first || key < c.keep)) atomicOr(p.err, KVB_DEV_BAD_PAGE);
+            return -1;
+        };
+        // Copies of a tile's keys and of both scale bytes, and of its values: one group each.
+        auto fetch_keys = [&](int i, int stage, const Pages& pages) {
             if (i < end) {
                 const int key0 = key_of(i);
                 const uint32_t base = slots + stage * STAGE_BYTES;
-                const bool all = key0 + WARP_KEYS - 1 <= pos_last && key0 >= lo_first;
-                auto seen = [&](int key) { return all || (key <= pos_last && (key >= lo_first || key < c.keep)); };
+                const bool all = key0 + UNIT - 1 <= pos_last && key0 >= lo_first;
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const bool has_k = row_k[s] >= 0, has_v = row_v[s] >= 0;
-                    const int at_k = has_k ? row_k[s] : 0, at_v = has_v ? row_v[s] : 0;
-                    const uint8_t* const from_k = k_lane + (size_t)(at_k + (g & 1)) * D;
-                    const uint8_t* const from_v = v_lane + (size_t)at_v * D;
+                    const int key = key0 + 16 * s + key_k, row = row_of(pages.k[s], key - (g & 1)), at = max(row, 0);
+                    const uint8_t* const from = k_lane + (size_t)(at + (g & 1)) * D;
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        const bool there = has_k && seen(key0 + 16 * s + key_k + 2 * n);
+                        const bool there = row >= 0 && (all || (key + 2 * n <= pos_last && (key + 2 * n >= lo_first || key + 2 * n < c.keep)));
 #pragma unroll
                         for (int u = 0; u < KN; ++u)
-                            copy_async<KU>(base + (((s * 2 + n) * KN + u) * 32 + lane) * KU, from_k + 2 * n * D + u * 4 * KU, there);
+                            copy_async<KU>(base + (((s * 2 + n) * KN + u) * 32 + lane) * KU, from + 2 * n * D + u * 4 * KU, there);
                     }
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4) {
-                        const bool there = has_v && seen(key0 + 16 * s + key_v + i4);
-#pragma unroll
-                        for (int u = 0; u < VN; ++u)
-                            copy_async<VU>(base + K_BYTES + (((s * 4 + i4) * VN + u) * 32 + lane) * VU, from_v + i4 * D + u * 8 * VU, there);
-                    }
-                    copy_async<4>(base + K_BYTES + V_BYTES + (2 * s * 32 + lane) * 4, p.k_scales + at_k, has_k);
-                    copy_async<4>(base + K_BYTES + V_BYTES + ((2 * s + 1) * 32 + lane) * 4, p.v_scales + at_k, has_k);
+                    copy_async<4>(base + K_BYTES + V_BYTES + (2 * s * 32 + lane) * 4, p.k_scales + at, row >= 0);
+                    copy_async<4>(base + K_BYTES + V_BYTES + ((2 * s + 1) * 32 + lane) * 4, p.v_scales + at, row >= 0);
                 }
             }
             copies_commit();
         };
-        lookup(begin);
+        auto fetch_values = [&](int i, int stage, const Pages& pages) {
+            if (i < end) {
+                const int key0 = key_of(i);
+                const uint32_t base = slots + stage * STAGE_BYTES + K_BYTES;
+                const bool all = key0 + UNIT - 1 <= pos_last && key0 >= lo_first;
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) { fetch(begin + s, s); lookup(begin + s + 1); }
+                for (int s = 0; s < 2; ++s) {
+                    const int key = key0 + 16 * s + key_v, row = row_of(pages.v[s], key);
+                    const uint8_t* const from = v_lane + (size_t)max(row, 0) * D;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const bool there = row >= 0 && (all || (key + n <= pos_last && (key + n >= lo_first || key + n < c.keep)));
+#pragma unroll
+                        for (int u = 0; u < VN; ++u)
+                            copy_async<VU>(base + (((s * 4 + n) * VN + u) * 32 + lane) * VU, from + n * D + u * 8 * VU, there);
+                    }
+                }
+            }
+            copies_commit();
+        };
+        const int mine_first = begin + warp;                 // the warps take tiles in turn
+        Pages ahead[STAGES], next;
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) ahead[s] = lookup(mine_first + s * WARPS);
+        next = lookup(mine_first + STAGES * WARPS);          // always a tile before its pages are looked at
+        // This lane's numbers of query row 8 j + g: D / 4 of them, KU together.
+        constexpr int QN = D / 4 / 8;                        // 16 bytes at a time
+        uint4 raw[ROW_TILES][QN];
+#pragma unroll
+        for (int j = 0; j < ROW_TILES; ++j) {
+            const int row = row0 + 8 * j + g, token = row / p.group, head = hk * p.group + row - token * p.group;
+            const bf16* const from = p.q + ((size_t)(c.q_start + token) * p.Hq + head) * D + t * KU;
+#pragma unroll
+            for (int k = 0; k < QN; ++k)
+                raw[j][k] = 8 * j + g < rows ? *reinterpret_cast<const uint4*>(from + (k / (KU / 8)) * 4 * KU + (k % (KU / 8)) * 8) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) {
+            fetch_keys(mine_first + s * WARPS, s, ahead[s]);
+            fetch_values(mine_first + s * WARPS, s, ahead[s]);
+        }
 
         // Queries as fragments, brought to about 1 by a power of two that goes into the score's factor: this lane holds numbers of row
         // 8 j + g, and the scores of rows 8 j + 2 t and the next.
-        uint32_t qf[ROW_TILES][KN * KU / 4][2];
+        uint32_t qf[ROW_TILES][2][QN][2];                    // [eight of rows][high or low part][32 numbers of a head]
         float factor[ROW_TILES][2], slope[ROW_TILES][2];
         int pos[ROW_TILES][2], lo[ROW_TILES][2];
         const bool biased = p.cap > 0.f || p.slopes;
 #pragma unroll
         for (int j = 0; j < ROW_TILES; ++j) {
-            const int row = row0 + 8 * j + g, token = row / p.group, head = hk * p.group + row - token * p.group;
-            const bool there = 8 * j + g < rows;
-            uint2 raw[KN * KU / 4];
             uint32_t top = 0u;
-            const bf16* const from = p.q + ((size_t)(c.q_start + token) * p.Hq + head) * D + t * KU;
 #pragma unroll
-            for (int k = 0; k < KN * KU / 4; ++k) {
-                raw[k] = there ? *reinterpret_cast<const uint2*>(from + (k / (KU / 4)) * 4 * KU + (k % (KU / 4)) * 4) : make_uint2(0u, 0u);
-                top = max(top, max(max(raw[k].x & 0x7fffu, (raw[k].x >> 16) & 0x7fffu), max(raw[k].y & 0x7fffu, (raw[k].y >> 16) & 0x7fffu)));
+            for (int k = 0; k < QN; ++k) {
+                const uint32_t x[4] = {raw[j][k].x, raw[j][k].y, raw[j][k].z, raw[j][k].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
             }
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int e = top == 0u || top >= 0x7f80u ? 0 : min(100, max(-100, (int)(top >> 7) - 127));
-            const float down = __int_as_float((127 - e) << 23), up = __int_as_float((127 + e) << 23);
+            const float down = __int_as_float((127 - e) << 23), up = top >= 0x7f80u ? __int_as_float(0x7fffffff) : __int_as_float((127 + e) << 23);
 #pragma unroll
-            for (int k = 0; k < KN * KU / 4; ++k) {          // the pairs of a word that `halves` makes
-                qf[j][k][0] = pack(__uint_as_float(raw[k].x << 16) * down, __uint_as_float(raw[k].y << 16) * down);
-                qf[j][k][1] = pack(__uint_as_float(raw[k].x & 0xffff0000u) * down, __uint_as_float(raw[k].y & 0xffff0000u) * down);
+            for (int k = 0; k < QN; ++k) {
+                const uint32_t x[4] = {raw[j][k].x, raw[j][k].y, raw[j][k].z, raw[j][k].w};
+                uint32_t high[4], low[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    split_queries<STORE>(__uint_as_float(x[i] << 16) * down, __uint_as_float(x[i] & 0xffff0000u) * down, high[i], low[i]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    qf[j][0][k][i] = high[2 * i] | high[2 * i + 1] << 16;
+                    qf[j][1][k][i] = low[2 * i] | low[2 * i + 1] << 16;
+                }
             }
 #pragma unroll
             for (int e2 = 0; e2 < 2; ++e2) {
@@ -305,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
                 pos[j][e2] = r < rows ? c.start + token2 : 0;
                 lo[j][e2] = first_seen_key(pos[j][e2], p.reach);
                 slope[j][e2] = r < rows && p.slopes ? p.slopes[hk * p.group + row0 + r - token2 * p.group] : 0.f;
-                factor[j][e2] = p.scale * CODE_SCALE<STORE> * __shfl_sync(0xffffffffu, up, 4 * (2 * t + e2)) * (biased ? 1.f : 1.4426950408889634f);
+                factor[j][e2] = p.scale * QUERY_SCALE<STORE> * __shfl_sync(0xffffffffu, up, 4 * (2 * t + e2)) * (biased ? 1.f : 1.4426950408889634f);
             }
         }
 
@@ -319,16 +417,21 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
             l[j][0] = l[j][1] = 0.f;
         }
 
-        // 32 keys from `key0` on, whose bytes are there.  MASKED: some row may miss one of them.
-        auto tile = [&](int key0, int stage, auto masked_tag) {
-            constexpr bool MASKED = decltype(masked_tag)::value;
+        // Tile i, whose slots are those of `stage`; a slot is filled anew, STAGES tiles ahead, as soon as it has been read.  MASKED: some row may
+        // miss a key of it.
+        auto tile = [&](int i, int stage, auto masked_tag, auto biased_tag) {
+            const int key0 = key_of(i);
+            constexpr bool MASKED = decltype(masked_tag)::value, BIASED = decltype(biased_tag)::value;
             const uint32_t base = slots + stage * STAGE_BYTES;
+            copies_wait<2 * STAGES - 1>();
             float s[2][ROW_TILES][4];                        // [half][eight of rows][key row g or g + 8, query row]
-            uint32_t kb[2], vb[2];
+            uint32_t kb[2], vb[2], part[2][2][ROW_TILES][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int j = 0; j < ROW_TILES; ++j) s[h][j][0] = s[h][j][1] = s[h][j][2] = s[h][j][3] = 0.f;
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int j = 0; j < ROW_TILES; ++j) part[h][x][j][0] = part[h][x][j][1] = part[h][x][j][2] = part[h][x][j][3] = 0u;
                 read_slot<4>(base + K_BYTES + V_BYTES + (2 * h * 32 + lane) * 4, &kb[h]);
                 read_slot<4>(base + K_BYTES + V_BYTES + ((2 * h + 1) * 32 + lane) * 4, &vb[h]);
             }
@@ -340,82 +443,86 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
 #pragma unroll
                     for (int n = 0; n < 2; ++n) read_slot<KU>(base + (((h * 2 + n) * KN + u) * 32 + lane) * KU, word[n]);
 #pragma unroll
-                    for (int k = 0; k < KU / 4; ++k) {
-                        uint32_t a[4];
-                        halves<STORE>(word[0][k], a[0], a[2]);
-                        halves<STORE>(word[1][k], a[1], a[3]);
+                    for (int k = 0; k < KU / 8; ++k)
 #pragma unroll
-                        for (int j = 0; j < ROW_TILES; ++j) mma(s[h][j], a[0], a[1], a[2], a[3], qf[j][u * (KU / 4) + k]);
-                    }
+                        for (int j = 0; j < ROW_TILES; ++j)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                mma8<STORE>(part[h][x][j], word[0][2 * k], word[1][2 * k], word[0][2 * k + 1], word[1][2 * k + 1], qf[j][x][u * (KU / 8) + k]);
                 }
-            // Exponents of the weights that the value codes get: score (base 2) + the value row's exponent.
-            float top[ROW_TILES][2], inv[2][2];
-            uint32_t hidden = 0u;                            // (MASKED) a bit a score
 #pragma unroll
-            for (int j = 0; j < ROW_TILES; ++j) top[j][0] = top[j][1] = NEG_INF;
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < ROW_TILES; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[h][j][e] = joined<STORE>(part[h][0][j][e], part[h][1][j][e]);
+            fetch_keys(i + STAGES * WARPS, stage, next);
+            // Exponents of the weights that the value codes get: score (base 2) + the value row's exponent.
+            float inv[2][2];
+            uint32_t hidden = 0u;                            // (MASKED) a bit a score
+            bool above = false;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    const int at_byte = 8 * ((g & 1) + 2 * n);
-                    const int kbyte = (kb[h] >> at_byte) & 255, vbyte = (vb[h] >> at_byte) & 255;
-                    const float up = __int_as_float(kbyte << 23);
-                    const float shift = __int_as_float(0x4b000000 | vbyte) - 8388735.f;           // vbyte - 127
-                    inv[h][n] = __int_as_float((254 - vbyte) << 23);                              // -infinity for a row that is not finite
+                    const uint32_t pick = n ? pick_second : pick_first;
+                    const float up = __uint_as_float(__byte_perm(kb[h], 0u, pick) >> 1);                             // byte << 23
+                    const float shift = __uint_as_float(__byte_perm(vb[h], 0x4b000000u, 0x7550u | (pick >> 12))) - 8388735.f;      // byte - 127
+                    inv[h][n] = __uint_as_float(0x7f000000u - (__byte_perm(vb[h], 0u, pick) >> 1));                  // -infinity for a row that is not finite
                     const int key = key0 + 16 * h + key_k + 2 * n;
 #pragma unroll
                     for (int j = 0; j < ROW_TILES; ++j)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float x = s[h][j][2 * n + e] * up * factor[j][e];
-                            if (biased) {
+                            float x = s[h][j][2 * n + e];
+                            if (BIASED) {
+                                x = x * up * factor[j][e];
                                 if (p.cap > 0.f) x = p.cap * (1.f - __fdividef(2.f, 1.f + ex2(x / p.cap * 2.885390081777927f)));
-                                x = (x - slope[j][e] * (float)(pos[j][e] - key)) * 1.4426950408889634f;
+                                x = fmaf(x - slope[j][e] * (float)(pos[j][e] - key), 1.4426950408889634f, shift);
+                            } else {
+                                x = fmaf(x, up * factor[j][e], shift);
                             }
-                            x += shift;
                             if (MASKED && !(key <= pos[j][e] && (key >= lo[j][e] || key < c.keep))) {
                                 x = NEG_INF;
                                 hidden |= 1u << (((2 * h + n) * ROW_TILES + j) * 2 + e);
                             }
                             s[h][j][2 * n + e] = x;
-                            top[j][e] = fmaxf(top[j][e], x);
+                            above |= x > m[j][e] + HEADROOM;
                         }
                 }
-            bool moved = false;
-            float base_m[ROW_TILES][2], corr[ROW_TILES][2];
+            // The reference that weights are taken against follows a row's maximum only when that has moved by 2^HEADROOM, far below half
+            // precision's 2^16: then the row's lanes agree on it and what has been added up is rescaled.
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int j = 0; j < ROW_TILES; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(fmaxf(s[0][j][e], s[0][j][2 + e]), fmaxf(s[1][j][e], s[1][j][2 + e]));
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        const float now = fmaxf(m[j][e], top);
+                        const float corr = ex2(m[j][e] - (now == NEG_INF ? 0.f : now));
+                        m[j][e] = now;
+                        l[j][e] *= corr;
+#pragma unroll
+                        for (int i = 0; i < VN * VU / 2; ++i) { o[j][i][e] *= corr; o[j][i][2 + e] *= corr; }
+                    }
+            }
 #pragma unroll
             for (int j = 0; j < ROW_TILES; ++j)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
+                    const float base_m = MASKED && m[j][e] == NEG_INF ? 0.f : m[j][e];
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) top[j][e] = fmaxf(top[j][e], __shfl_xor_sync(0xffffffffu, top[j][e], x));
-                    const float now = fmaxf(m[j][e], top[j][e]);
-                    base_m[j][e] = now == NEG_INF ? 0.f : now;
-                    corr[j][e] = ex2(m[j][e] - base_m[j][e]);
-                    moved |= now > m[j][e];
-                    m[j][e] = now;
-                    l[j][e] *= corr[j][e];
-                }
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int j = 0; j < ROW_TILES; ++j)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
+                        for (int n = 0; n < 2; ++n) {
                             float& x = s[h][j][2 * n + e];
-                            x = ex2(x - base_m[j][e]);
+                            x = ex2(x - base_m);
                             l[j][e] = fmaf(x, MASKED && ((hidden >> (((2 * h + n) * ROW_TILES + j) * 2 + e)) & 1u) ? 0.f : inv[h][n], l[j][e]);
                         }
-            if (__any_sync(0xffffffffu, moved)) {            // the maxima seldom move once a few tiles are in
-#pragma unroll
-                for (int j = 0; j < ROW_TILES; ++j)
-#pragma unroll
-                    for (int i = 0; i < VN * VU / 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][i][e] *= corr[j][e & 1];
-            }
+                }
+            copies_wait<2 * STAGES - 1>();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 uint32_t pf[ROW_TILES][2];
@@ -444,16 +551,17 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         };
 
         int stage = 0;
-        for (int i = begin; i < end; ++i) {
-            // The slots that the next fetch fills were read by this lane alone, in the turn before.
+        for (int i = mine_first; i < end; i += WARPS) {
             const int key0 = key_of(i);
-            fetch(i + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
-            lookup(i + STAGES);
-            copies_wait<STAGES - 1>();
-            if (key0 <= pos_last && (key0 + WARP_KEYS > lo_first || key0 < c.keep)) {
-                if (key0 + WARP_KEYS - 1 <= pos_first && key0 >= lo_last) tile(key0, stage, std::false_type{});
-                else tile(key0, stage, std::true_type{});
-            }
+            const Pages after = lookup(i + (STAGES + 1) * WARPS);
+            if (key0 > pos_last || (key0 + UNIT <= lo_first && key0 >= c.keep)) {      // the segment's other rows see it
+                copies_wait<2 * STAGES - 2>();
+                fetch_keys(i + STAGES * WARPS, stage, next);
+            } else if (biased) tile(i, stage, std::true_type{}, std::true_type{});
+            else if (key0 + UNIT - 1 <= pos_first && key0 >= lo_last) tile(i, stage, std::false_type{}, std::false_type{});
+            else tile(i, stage, std::true_type{}, std::false_type{});
+            fetch_values(i + STAGES * WARPS, stage, next);
+            next = after;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
         copies_wait<0>();
@@ -479,8 +587,8 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
                 if (g == 0) { ml_s[2 * r] = m[j][e]; ml_s[2 * r + 1] = l[j][e]; }
             }
         __syncthreads();
-        const int block0 = item_first / share, block1 = (item_first + c.n - 1) / share;
-        auto place_of = [&](int b) -> size_t { return (size_t)2 * b + (b * share > item_first ? 0 : 1); };
+        // A block's places: of a row tile that another block has begun, and of one that it leaves to others.
+        auto place_of = [&](int b) -> size_t { return (size_t)2 * b + (b > block0 ? 0 : 1); };
         auto store_row = [&](int r, int col, float4 x, float M, float L) {
             const int row = row0 + r, token = row / p.group, head = hk * p.group + row - token * p.group;
             if (p.sink) L += ex2(p.sink[head] * 1.4426950408889634f - (M == NEG_INF ? 0.f : M));
@@ -516,60 +624,63 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
             }
         }
         if (block0 != block1) {
-            // Adds what blocks b0 .. b1 (every `step`th) have left, in order: (row, columns, sums, m, l) go to `put`, after all have been read.
-            auto add_up = [&](int b0, int b1, int step, auto put) {
-                float* const ml_all = reinterpret_cast<float*>(smem);        // weights, m and l of up to GROUP pieces
-                const int n = (b1 - b0) / step + 1;
-                for (int idx = tid; idx < rows * n; idx += THREADS) {
-                    const int k = idx / rows, r = idx - k * rows;
-                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (place_of(b0 + k * step) * ROWS + r) * 2));
-                    ml_all[2 * (r * GROUP + k)] = ml.x;
-                    ml_all[2 * (r * GROUP + k) + 1] = ml.y;
-                }
-                __syncthreads();
-                for (int i0 = 0; i0 < rows * (D / 4); i0 += THREADS) {
-                    const int idx = i0 + tid;
-                    const bool mine_too = idx < rows * (D / 4);
-                    const int r = mine_too ? idx / (D / 4) : 0, col = mine_too ? (idx - r * (D / 4)) * 4 : 0;
+            // Adds what n blocks from b0 on (every `step`th) have left, in order: (row, columns, sums, m, l) go to `put`.  A warp takes its rows by
+            // itself, with the loads of CHUNK pieces in flight; little code, which only a few blocks meet, and cold.
+            auto add_up = [&](int b0, int n, int step, auto put) {
+                constexpr int QUADS = D / 4, AT_ONCE = 32 / QUADS, CHUNK = 8;
+#pragma unroll 1
+                for (int r0 = warp * AT_ONCE; r0 < rows; r0 += WARPS * AT_ONCE) {
+                    const int r = r0 + lane / QUADS, col = lane % QUADS * 4;
+                    const bool there = lane < AT_ONCE * QUADS && r < rows;
                     float M = NEG_INF, L = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int k = 0; k < n; ++k) M = fmaxf(M, ml_all[2 * (r * GROUP + k)]);
-                    const float base_m = M == NEG_INF ? 0.f : M;
 #pragma unroll 1
-                    for (int k0 = 0; k0 < n; k0 += 4) {
-                        float4 y[4];
+                    for (int k0 = 0; k0 < n; k0 += CHUNK) {
+                        float2 ml[CHUNK];
+                        float4 y[CHUNK];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (k0 + k < n) y[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (place_of(b0 + (k0 + k) * step) * ROWS + r) * D + col));
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (k0 + k < n) {
-                                const float f = ex2(ml_all[2 * (r * GROUP + k0 + k)] - base_m);
-                                L = fmaf(f, ml_all[2 * (r * GROUP + k0 + k) + 1], L);
-                                x.x = fmaf(f, y[k].x, x.x); x.y = fmaf(f, y[k].y, x.y); x.z = fmaf(f, y[k].z, x.z); x.w = fmaf(f, y[k].w, x.w);
+                        for (int k = 0; k < CHUNK; ++k) {
+                            ml[k] = make_float2(NEG_INF, 0.f);
+                            y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (there && k0 + k < n) {
+                                const size_t at = place_of(b0 + (k0 + k) * step) * ROWS + r;
+                                ml[k] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + at);
+                                y[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + col));
                             }
+                        }
+                        float now = M;
+#pragma unroll
+                        for (int k = 0; k < CHUNK; ++k) now = fmaxf(now, ml[k].x);
+                        const float base_m = now == NEG_INF ? 0.f : now, corr = ex2(M - base_m);
+                        M = now;
+                        L *= corr;
+                        x.x *= corr; x.y *= corr; x.z *= corr; x.w *= corr;
+#pragma unroll
+                        for (int k = 0; k < CHUNK; ++k) {
+                            const float f = ex2(ml[k].x - base_m);
+                            L = fmaf(f, ml[k].y, L);
+                            x.x = fmaf(f, y[k].x, x.x); x.y = fmaf(f, y[k].y, x.y); x.z = fmaf(f, y[k].z, x.z); x.w = fmaf(f, y[k].w, x.w);
+                        }
                     }
-                    if (mine_too) put(r, col, x, M, L);
+                    __syncwarp();                            // all of the row has been read
+                    if (there) put(r, col, x, M, L);
                 }
-                __syncthreads();
             };
             // The last of `of` blocks to raise a ticket, which it sets back.
             auto last_of = [&](int* ticket, int of) -> bool {
-                __threadfence();
                 __syncthreads();
                 if (tid == 0) {
-                    ticket_s = atomicAdd(ticket, 1);
+                    // The barrier orders the block's stores before this, and what the others released before the block's reads.
+                    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;\n" : "=r"(ticket_s) : "l"(ticket) : "memory");
                     if (ticket_s == of - 1) *ticket = 0;
                 }
                 __syncthreads();
-                const bool last = ticket_s == of - 1;
-                if (last) __threadfence();
-                return last;
+                return ticket_s == of - 1;
             };
-            // Pieces are added in groups of GROUP neighbours, the groups' sums (which lie where their first pieces' lay) in groups again.
+            // More than MOST pieces are added in groups of GROUP neighbours, the groups' sums (which lie where their first pieces' lay) in groups again.
             bool last = true;
             int step = 1;
-            for (; last && (block1 - block0) / step >= GROUP; step *= GROUP) {
+            for (; last && (block1 - block0) / step >= MOST; step *= GROUP) {
                 const int b0 = block0 + ((int)blockIdx.x - block0) / (step * GROUP) * (step * GROUP);
                 const int members = min(GROUP, (block1 - b0) / step + 1);
                 // A block leads a group of one item that starts in it and of one that goes through it, of each size.
@@ -577,14 +688,14 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
                 if (last) {
                     float* const to_o = p.part_o + place_of(b0) * ROWS * D;
                     float* const to_ml = p.part_ml + place_of(b0) * ROWS * 2;
-                    add_up(b0, b0 + (members - 1) * step, step, [&](int r, int col, float4 x, float M, float L) {
+                    add_up(b0, members, step, [&](int r, int col, float4 x, float M, float L) {
                         *reinterpret_cast<float4*>(to_o + r * D + col) = x;
                         if (col == 0) *reinterpret_cast<float2*>(to_ml + r * 2) = make_float2(M, L);
                     });
                 }
             }
             if (last && last_of(p.tickets + (size_t)6 * gridDim.x + block0, (block1 - block0) / step + 1))
-                add_up(block0, block0 + (block1 - block0) / step * step, step, store_row);
+                add_up(block0, (block1 - block0) / step + 1, step, store_row);
         }
         __syncthreads();                                     // the slots are the next piece's
     }

@@ -976,7 +976,7 @@ class CudaKernels(KernelSet):
     # Bytes of keys and values that a layer reads back for a step's portions; longer ones read the codes in place.
     CACHE_EXPAND_MAX_BYTES = 1 << 30
     quant_expand_min_rows = 64           # portions of at least this many tokens have their keys and values read back first
-    quant_min_units = 2                  # units of 128 keys a block of csrc/attention_quant.cu takes at least
+    quant_min_units = 8                  # units of 32 keys a block of csrc/attention_quant.cu takes at least
 
     def _quant_library(self, head_dim: int) -> Tuple[_Library, int, int]:
         """(the kernels, floats of scratch, tickets)"""
