@@ -48,7 +48,7 @@ constexpr int O_STRIDE = D + 4;
 template <int ROW_TILES> constexpr int blocks_per_sm() { return ROW_TILES == 1 ? (D <= 64 ? 4 : 3) : ROW_TILES == 2 ? (D <= 64 ? 3 : 2) : 2; }
 constexpr int MAX_SEGMENTS = 4096;
 constexpr int GROUP = 16, MOST = 32;   // pieces whose sums one block adds up: of a group, and of the last ones that are left
-constexpr int PIECE_COST = 4;          // what a piece costs beside its keys, in units
+constexpr int PIECE_COST = 7;          // what a piece costs beside its keys, in units
 constexpr float NEG_INF = -INFINITY;
 constexpr float HEADROOM = 8.f;
 
@@ -141,23 +141,21 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
 }
-// A word of four codes as half precision: its bytes 0 and 2, and its bytes 1 and 3.  An e4m3 number's exponent and mantissa are put where
-// half precision has them, which makes it 2^-8 times as large (CODE_SCALE), subnormal ones included: seven instructions, where
-// the conversion instruction takes fourteen for four codes.  An int8 code with its sign bit flipped becomes the low bits of 1024 + c + 128.
+// Two neighbouring codes, the lower or the upper two bytes of a word, as half precision.  An int8 code with its sign bit flipped becomes the
+// low bits of 1024 + c + 128.  (e4m3: two conversions take 6 clocks a word and scheduler, putting exponent and mantissa where half
+// precision has them by shifts and masks 10.)
 template <int STORE>
-__device__ __forceinline__ void halves(uint32_t w, uint32_t& even, uint32_t& odd) {
+__device__ __forceinline__ void halves(uint32_t w, uint32_t& lower, uint32_t& upper) {
     if (STORE == KVB_INT8) {
+        const uint32_t f = w ^ 0x80808080u, a = __byte_perm(f, 0x64646464u, 0x4140), b = __byte_perm(f, 0x64646464u, 0x4342);
         const __half2 off = __half2half2(__ushort_as_half(0x6480));          // 1152
-        const uint32_t a = (w & 0x00ff00ffu) ^ 0x64806480u, b = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
         const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off), y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-        even = *reinterpret_cast<const uint32_t*>(&x);
-        odd = *reinterpret_cast<const uint32_t*>(&y);
+        lower = *reinterpret_cast<const uint32_t*>(&x);
+        upper = *reinterpret_cast<const uint32_t*>(&y);
     } else {
-        even = ((w << 7) & 0x3f803f80u) | ((w << 8) & 0x80008000u);
-        odd = ((w >> 1) & 0x3f803f80u) | (w & 0x80008000u);
+        asm("{.reg .b16 x, y; mov.b32 {x, y}, %2; cvt.rn.f16x2.e4m3x2 %0, x; cvt.rn.f16x2.e4m3x2 %1, y;}" : "=r"(lower), "=r"(upper) : "r"(w));
     }
 }
-template <int STORE> constexpr float CODE_SCALE = STORE == KVB_E4M3 ? 256.f : 1.f;
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -541,8 +539,8 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {        // two columns of four keys
                             uint32_t a[4];
-                            halves<STORE>(__byte_perm(v[0][k], v[1][k], x ? 0x7632 : 0x5410), a[0], a[1]);
-                            halves<STORE>(__byte_perm(v[2][k], v[3][k], x ? 0x7632 : 0x5410), a[2], a[3]);
+                            halves<STORE>(__byte_perm(v[0][k], v[1][k], x ? 0x7362 : 0x5140), a[0], a[1]);
+                            halves<STORE>(__byte_perm(v[2][k], v[3][k], x ? 0x7362 : 0x5140), a[2], a[3]);
 #pragma unroll
                             for (int j = 0; j < ROW_TILES; ++j) mma(o[j][u * (VU / 2) + 2 * k + x], a[0], a[1], a[2], a[3], pf[j]);
                         }
@@ -592,7 +590,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         auto store_row = [&](int r, int col, float4 x, float M, float L) {
             const int row = row0 + r, token = row / p.group, head = hk * p.group + row - token * p.group;
             if (p.sink) L += ex2(p.sink[head] * 1.4426950408889634f - (M == NEG_INF ? 0.f : M));
-            const float k = L > 0.f ? CODE_SCALE<STORE> / L : L == 0.f ? 0.f : __int_as_float(0x7fffffff);
+            const float k = L > 0.f ? 1.f / L : L == 0.f ? 0.f : __int_as_float(0x7fffffff);
             __nv_bfloat162 a = __floats2bfloat162_rn(x.x * k, x.y * k), b = __floats2bfloat162_rn(x.z * k, x.w * k);
             *reinterpret_cast<uint2*>(p.out + ((size_t)(c.q_start + token) * p.Hq + head) * D + col) =
                 make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
