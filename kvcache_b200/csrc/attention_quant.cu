@@ -15,9 +15,10 @@
 // ROW_TILES eights of rows.  (Queries as the 16 rows: twice the MMAs and sums in registers for seven heads.)
 // A warp takes 32 keys at a time - a block's four in turn - and needs nothing from any other until the block's run ends.  The order of an MMA's inner index, and of its
 // rows, is free as long as all agree, so a lane's share of a tile is bytes that lie together: for the scores 16 (or 8) of a key's
-// numbers, for the sum the same of four neighbouring keys' values.  Each lane copies those bytes itself (cp.async, into slots of
-// shared memory that no other lane touches), two tiles ahead, and turns them into half precision in registers: no barrier, no
-// bank conflict and no wait for another lane stands in the stream.
+// numbers, for the sum the same of four neighbouring keys' values.  The warp copies its tiles itself, two ahead (cp.async: 512 bytes
+// that lie together with every instruction - with each lane copying what it will read, from 64 bytes a row, the stream alone took 80 us
+// where it now takes 58, 64 requests of 28 heads of 128 and 8,192 keys at most), into rows whose 16-byte parts are turned so that neither the
+// copies nor the reads meet a bank twice.  No barrier of the block stands in the stream.
 //
 // Work is shared out by keys: units of 32 keys of every (segment, key head, tile of rows), laid end to end, are cut into equal
 // runs, one a block, whatever the lengths.  Where a cut divides a row tile's keys, the pieces' sums meet in scratch, two places a
@@ -38,12 +39,14 @@ constexpr int D = KVB_HEAD_DIM;
 static_assert(D == 32 || D == 64 || D == 96 || D == 128, "head sizes 32, 64, 96 and 128");
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int UNIT = 32;                // keys a warp takes at a time
-constexpr int KU = D % 64 == 0 ? 16 : 8, KN = D / (4 * KU);                       // bytes a copy, copies a key row and lane: four lanes share a key row
-constexpr int VU = D % 128 == 0 ? 16 : D % 64 == 0 ? 8 : 4, VN = D / (8 * VU);    // ... eight lanes share a value row
-constexpr int K_BYTES = 4 * KN * KU * 32, V_BYTES = 8 * VN * VU * 32, STAGE_BYTES = K_BYTES + V_BYTES + 4 * 32 * 4;
-constexpr int STAGES = 2;
-constexpr int WARP_BYTES = STAGES * STAGE_BYTES;
+constexpr int KU = D % 64 == 0 ? 16 : 8, KN = D / (4 * KU);                       // bytes a read, reads of a key row by one of the four lanes that share it
+constexpr int VU = D % 128 == 0 ? 16 : D % 64 == 0 ? 8 : 4, VN = D / (8 * VU);    // ... of a value row by one of eight
+constexpr int K_BYTES = UNIT * D, STAGE_BYTES = 2 * K_BYTES + 64;                 // keys, values, and both scale bytes of a tile
+constexpr int STAGES = D <= 64 ? 3 : 2;
 constexpr int O_STRIDE = D + 4;
+// A warp's shared memory: its tiles, and over them its sums when a piece ends.
+template <int ROW_TILES>
+constexpr int warp_bytes = STAGES * STAGE_BYTES > 8 * ROW_TILES * (O_STRIDE * 4 + 8) ? STAGES * STAGE_BYTES : 8 * ROW_TILES * (O_STRIDE * 4 + 8);
 // Blocks an SM holds of the kernel for ROW_TILES eights of rows: registers allow 3 of 168 a thread, or 4 of 128, or 2 of 255.
 template <int ROW_TILES> constexpr int blocks_per_sm() { return ROW_TILES == 1 ? (D <= 64 ? 4 : 3) : ROW_TILES == 2 ? (D <= 64 ? 3 : 2) : 2; }
 constexpr int MAX_SEGMENTS = 4096;
@@ -84,6 +87,7 @@ template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, con
     if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(n) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(to), "l"(from), "n"(BYTES), "r"(n) : "memory");
 }
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 template <int BYTES> __device__ __forceinline__ void read_slot(uint32_t from, uint32_t* w) {
@@ -91,6 +95,37 @@ template <int BYTES> __device__ __forceinline__ void read_slot(uint32_t from, ui
     else if (BYTES == 8) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(from) : "memory");
     else asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[0]) : "r"(from) : "memory");
 }
+// Where a half tile's numbers lie in shared memory, as a lane sees it.  A row is D bytes in 16-byte parts.  Heads of 128: the eight parts of row
+// `key` are turned, part c lies at c ^ 2 ((key / 4) % 4) ^ 4 (key % 2).  Heads of 64: the four parts, c ^ 2 (key / 8), and rows 2 i and 2 i + 1
+// change places where key / 4 is odd.  Others: as they come.
+struct Lane {
+    int copy;        // copy f of 512 bytes: at 512 f + (copy ^ 32 f) with turned parts, else 512 f + copy
+    int k;           // key row g, this lane's first part: the next (heads of 128) at k ^ 64, of the others 4 KU further; key row g + 8: 2 D further
+    int v[2];        // values of keys 4 t and 4 t + 1; of 4 t + 2 and 4 t + 3: 2 D further
+};
+__device__ __forceinline__ Lane lane_places(int lane) {
+    const int g = lane >> 2, t = lane & 3, key = 4 * (g >> 1) + (g & 1);
+    Lane x;
+    if (D == 128) {
+        x.copy = (lane >> 3) * 128 + (((lane & 7) ^ (4 * ((lane >> 3) & 1))) << 4);
+        x.k = key * 128 + ((t ^ (2 * ((g >> 1) & 3)) ^ (4 * (g & 1))) << 4);
+        x.v[0] = t * 512 + ((g ^ (2 * t)) << 4);
+        x.v[1] = (x.v[0] ^ 64) + 128;
+    } else if (D == 64) {
+        x.copy = ((lane >> 2) ^ ((lane >> 4) & 1)) * 64 + ((lane & 3) << 4);
+        x.k = (key ^ ((g >> 1) & 1)) * 64 + ((t ^ (2 * (g >> 2))) << 4);
+        const int at = t * 256 + (((g >> 1) ^ (t & 2)) << 4) + (g & 1) * 8;
+        x.v[0] = at + 64 * (t & 1);
+        x.v[1] = at + 64 * (1 - (t & 1));
+    } else {
+        x.copy = lane * 16;
+        x.k = key * D + t * KU;
+        x.v[0] = t * 4 * D + g * VU;
+        x.v[1] = x.v[0] + D;
+    }
+    return x;
+}
+__device__ __forceinline__ int copy_place(const Lane& x, int f) { return 512 * f + (D % 64 == 0 && D != 96 ? x.copy ^ (32 * f) : x.copy); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -187,7 +222,7 @@ template <int STORE, int ROW_TILES>
 __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention_quant_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int ROWS = 8 * ROW_TILES;
-    static_assert(ROWS * O_STRIDE * 4 + ROWS * 8 <= WARP_BYTES, "a warp's sums lie over its slots");
+    constexpr int WARP_BYTES = warp_bytes<ROW_TILES>;
     int* const first = reinterpret_cast<int*>(smem + WARPS * WARP_BYTES);     // [segments + 1] the line before each segment
     __shared__ int ticket_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -233,13 +268,12 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
     unsigned char* const mine = smem + warp * WARP_BYTES;
     const uint32_t slots = smem_addr(mine);
     const int page_mask = (1 << p.page_shift) - 1;
+    const Lane at_lane = lane_places(lane);
     // Rows of an MMA are keys 4 (r / 2) + r % 2 for r < 8, and two further for r + 8: this lane's key rows are g and g + 8 of a tile of
     // 16, its values those of keys 4 t .. 4 t + 3.
-    const int key_k = 4 * (g >> 1) + (g & 1), key_v = 4 * t;
+    const int key_k = 4 * (g >> 1) + (g & 1);
     // Selectors that put the scale byte of key row g, or g + 8, of four neighbours' into a word's highest byte.
     const uint32_t pick_first = g & 1 ? 0x1444u : 0x0444u, pick_second = g & 1 ? 0x3444u : 0x2444u;
-    const uint8_t* const k_lane = p.k_codes + t * KU;
-    const uint8_t* const v_lane = p.v_codes + g * VU;
 
     for (int w = w_begin; w < w_end;) {
         while (first[seg + 1] <= w) ++seg;
@@ -272,80 +306,67 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         const int lo_first = first_seen_key(pos_first, p.reach), lo_last = first_seen_key(pos_last, p.reach);
         const int* const table = p.block_table + (size_t)seg * p.table_stride;
 
+        const int c_keep = c.keep;
         auto key_of = [&](int i) -> int { return (i < c.n_keep ? i : c.tile_begin - c.n_keep + i) * UNIT; };
-        // Pages of this lane's four neighbouring key rows and of its four values, of both halves of 32 keys, asked for one tile before
-        // they are looked at; -1: none that any row sees.
-        struct Pages { int k[2], v[2]; };
-        auto page_of = [&](int key) -> int {                 // of the four neighbouring keys from `key` on
+        // Pages of both halves of a tile, asked for one tile before they are looked at; -1: none that any row sees.  (Pages of fewer than 16
+        // tokens are looked up when they are wanted.)
+        struct Pages { int of[2]; };
+        auto page_of = [&](int key, int keys) -> int {       // of `keys` neighbours from `key` on
             const int place = key >> p.page_shift;
-            return key > pos_last || (key + 3 < lo_first && key >= c.keep) || place >= p.table_stride ? -1 : __ldg(table + place);
+            return key > pos_last || (key + keys <= lo_first && key >= c.keep) || place >= p.table_stride ? -1 : __ldg(table + place);
         };
         auto lookup = [&](int i) -> Pages {
-            Pages x = {{-1, -1}, {-1, -1}};
-            if (i < end) {
-                const int key0 = key_of(i);
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    x.k[s] = page_of(key0 + 16 * s + 4 * (g >> 1));
-                    x.v[s] = p.page_shift >= 4 && key0 + 16 * s + 15 <= pos_last && key0 + 16 * s >= lo_first ? x.k[s] : page_of(key0 + 16 * s + key_v);
-                }
-            }
-            return x;
+            if (i >= end || p.page_shift < 4) return {{-1, -1}};
+            const int key0 = key_of(i);
+            return {{page_of(key0, 16), page_of(key0 + 16, 16)}};
         };
-        // The pool's row of `key`, which lies in `page`; -1 without one, which is reported if some row sees the key.
-        auto row_of = [&](int page, int key) -> int {
+        // The pool's row of `key`, which lies in `page`; -1 without one, which is reported if some row sees one of the `keys` from it on.
+        auto row_of = [&](int page, int key, int keys) -> int {
             if (page >= 0 && page < p.num_pages) return ((page * p.Hkv + hk) << p.page_shift) + (key & page_mask);
-            if (key <= pos_last && (key + 3 >= lo_first || key < c.keep)) atomicOr(p.err, KVB_DEV_BAD_PAGE);
+            if (key <= pos_last && (key + keys > lo_first || key < c.keep)) atomicOr(p.err, KVB_DEV_BAD_PAGE);
             return -1;
         };
-        // Copies of a tile's keys and of both scale bytes, and of its values: one group each.
-        auto fetch_keys = [&](int i, int stage, const Pages& pages) {
-            if (i < end) {
-                const int key0 = key_of(i);
-                const uint32_t base = slots + stage * STAGE_BYTES;
-                const bool all = key0 + UNIT - 1 <= pos_last && key0 >= lo_first;
+        // Copies of a tile's keys with both scale bytes, and of its values: one group each.  Keys that no row sees become zeros.
+        auto fetch = [&](int i, uint32_t to, const uint8_t* codes, const Pages& pages) {
+            const int key0 = key_of(i);
+            if (key0 + UNIT - 1 <= pos_last && key0 >= lo_first && (unsigned)pages.of[0] < (unsigned)p.num_pages && (unsigned)pages.of[1] < (unsigned)p.num_pages) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const int key = key0 + 16 * s + key_k, row = row_of(pages.k[s], key - (g & 1)), at = max(row, 0);
-                    const uint8_t* const from = k_lane + (size_t)(at + (g & 1)) * D;
+                    const uint8_t* const from = codes + (size_t)(((pages.of[s] * p.Hkv + hk) << p.page_shift) + ((key0 + 16 * s) & page_mask)) * D + lane * 16;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const bool there = row >= 0 && (all || (key + 2 * n <= pos_last && (key + 2 * n >= lo_first || key + 2 * n < c.keep)));
-#pragma unroll
-                        for (int u = 0; u < KN; ++u)
-                            copy_async<KU>(base + (((s * 2 + n) * KN + u) * 32 + lane) * KU, from + 2 * n * D + u * 4 * KU, there);
-                    }
-                    copy_async<4>(base + K_BYTES + V_BYTES + (2 * s * 32 + lane) * 4, p.k_scales + at, row >= 0);
-                    copy_async<4>(base + K_BYTES + V_BYTES + ((2 * s + 1) * 32 + lane) * 4, p.v_scales + at, row >= 0);
+                    for (int f = 0; f < D / 32; ++f) copy_async(to + s * 16 * D + copy_place(at_lane, f), from + f * 512);
+                }
+            } else {                                         // edges, small pages, pages that are not there
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                    const int s = c / (D / 32), f = c - s * (D / 32), part = 32 * f + lane, in_half = part / (D / 16), key = key0 + 16 * s + in_half;
+                    const int row = row_of(p.page_shift >= 4 ? (s ? pages.of[1] : pages.of[0]) : page_of(key, 1), key, 1);
+                    const bool seen = row >= 0 && key <= pos_last && (key >= lo_first || key < c_keep);
+                    copy_async<16>(to + s * 16 * D + copy_place(at_lane, f), codes + (size_t)max(row, 0) * D + (part - in_half * (D / 16)) * 16, seen);
+                }
+            }
+        };
+        auto fetch_keys = [&](int i, int stage, const Pages& pages) {
+            if (i < end) {
+                const uint32_t to = slots + stage * STAGE_BYTES;
+                fetch(i, to, p.k_codes, pages);
+                if (lane < 16) {                             // four scale bytes a lane: of the first half's keys and values, then of the second's
+                    const int key = key_of(i) + 16 * (lane >> 3) + 4 * (lane & 3);
+                    const int row = row_of(p.page_shift >= 4 ? (lane & 8 ? pages.of[1] : pages.of[0]) : page_of(key, 4), key, 4);
+                    copy_async<4>(to + 2 * K_BYTES + lane * 4, (lane & 4 ? p.v_scales : p.k_scales) + max(row, 0), row >= 0);
                 }
             }
             copies_commit();
         };
         auto fetch_values = [&](int i, int stage, const Pages& pages) {
-            if (i < end) {
-                const int key0 = key_of(i);
-                const uint32_t base = slots + stage * STAGE_BYTES + K_BYTES;
-                const bool all = key0 + UNIT - 1 <= pos_last && key0 >= lo_first;
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const int key = key0 + 16 * s + key_v, row = row_of(pages.v[s], key);
-                    const uint8_t* const from = v_lane + (size_t)max(row, 0) * D;
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const bool there = row >= 0 && (all || (key + n <= pos_last && (key + n >= lo_first || key + n < c.keep)));
-#pragma unroll
-                        for (int u = 0; u < VN; ++u)
-                            copy_async<VU>(base + (((s * 4 + n) * VN + u) * 32 + lane) * VU, from + n * D + u * 8 * VU, there);
-                    }
-                }
-            }
+            if (i < end) fetch(i, slots + stage * STAGE_BYTES + K_BYTES, p.v_codes, pages);
             copies_commit();
         };
         const int mine_first = begin + warp;                 // the warps take tiles in turn
-        Pages ahead[STAGES], next;
+        // Pages are looked up a tile before they are wanted.
+        Pages ahead[STAGES + 1];
 #pragma unroll
-        for (int s = 0; s < STAGES; ++s) ahead[s] = lookup(mine_first + s * WARPS);
-        next = lookup(mine_first + STAGES * WARPS);          // always a tile before its pages are looked at
+        for (int s = 0; s <= STAGES; ++s) ahead[s] = lookup(mine_first + s * WARPS);
         // This lane's numbers of query row 8 j + g: D / 4 of them, KU together.
         constexpr int QN = D / 4 / 8;                        // 16 bytes at a time
         uint4 raw[ROW_TILES][QN];
@@ -357,11 +378,14 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
             for (int k = 0; k < QN; ++k)
                 raw[j][k] = 8 * j + g < rows ? *reinterpret_cast<const uint4*>(from + (k / (KU / 8)) * 4 * KU + (k % (KU / 8)) * 8) : make_uint4(0u, 0u, 0u, 0u);
         }
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < STAGES; ++s) {
-            fetch_keys(mine_first + s * WARPS, s, ahead[s]);
-            fetch_values(mine_first + s * WARPS, s, ahead[s]);
+            fetch_keys(mine_first + s * WARPS, s, ahead[0]);
+            fetch_values(mine_first + s * WARPS, s, ahead[0]);
+#pragma unroll
+            for (int x = 0; x < STAGES; ++x) ahead[x] = ahead[x + 1];
         }
+        Pages next = ahead[0];
 
         // Queries as fragments, brought to about 1 by a power of two that goes into the score's factor: this lane holds numbers of row
         // 8 j + g, and the scores of rows 8 j + 2 t and the next.
@@ -415,46 +439,11 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
             l[j][0] = l[j][1] = 0.f;
         }
 
-        // Tile i, whose slots are those of `stage`; a slot is filled anew, STAGES tiles ahead, as soon as it has been read.  MASKED: some row may
-        // miss a key of it.
-        auto tile = [&](int i, int stage, auto masked_tag, auto biased_tag) {
-            const int key0 = key_of(i);
-            constexpr bool MASKED = decltype(masked_tag)::value, BIASED = decltype(biased_tag)::value;
-            const uint32_t base = slots + stage * STAGE_BYTES;
-            copies_wait<2 * STAGES - 1>();
-            float s[2][ROW_TILES][4];                        // [half][eight of rows][key row g or g + 8, query row]
-            uint32_t kb[2], vb[2], part[2][2][ROW_TILES][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int j = 0; j < ROW_TILES; ++j) part[h][x][j][0] = part[h][x][j][1] = part[h][x][j][2] = part[h][x][j][3] = 0u;
-                read_slot<4>(base + K_BYTES + V_BYTES + (2 * h * 32 + lane) * 4, &kb[h]);
-                read_slot<4>(base + K_BYTES + V_BYTES + ((2 * h + 1) * 32 + lane) * 4, &vb[h]);
-            }
-#pragma unroll
-            for (int u = 0; u < KN; ++u)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t word[2][KU / 4];
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) read_slot<KU>(base + (((h * 2 + n) * KN + u) * 32 + lane) * KU, word[n]);
-#pragma unroll
-                    for (int k = 0; k < KU / 8; ++k)
-#pragma unroll
-                        for (int j = 0; j < ROW_TILES; ++j)
-#pragma unroll
-                            for (int x = 0; x < 2; ++x)
-                                mma8<STORE>(part[h][x][j], word[0][2 * k], word[1][2 * k], word[0][2 * k + 1], word[1][2 * k + 1], qf[j][x][u * (KU / 8) + k]);
-                }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < ROW_TILES; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[h][j][e] = joined<STORE>(part[h][0][j][e], part[h][1][j][e]);
-            fetch_keys(i + STAGES * WARPS, stage, next);
+        float s[2][ROW_TILES][4];                            // scores, then weights: [half][eight of rows][key row g or g + 8, query row]
+        // Weights of the tile from `key0` on, whose scale bytes are given, from its scores.  MASKED: some row may miss a key of it, or scores are capped or
+        // biased.
+        auto weigh = [&](int key0, const uint32_t (&kb)[2], const uint32_t (&vb)[2], auto masked_tag) {
+            constexpr bool MASKED = decltype(masked_tag)::value;
             // Exponents of the weights that the value codes get: score (base 2) + the value row's exponent.
             float inv[2][2];
             uint32_t hidden = 0u;                            // (MASKED) a bit a score
@@ -473,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             float x = s[h][j][2 * n + e];
-                            if (BIASED) {
+                            if (MASKED && biased) {
                                 x = x * up * factor[j][e];
                                 if (p.cap > 0.f) x = p.cap * (1.f - __fdividef(2.f, 1.f + ex2(x / p.cap * 2.885390081777927f)));
                                 x = fmaf(x - slope[j][e] * (float)(pos[j][e] - key), 1.4426950408889634f, shift);
@@ -520,44 +509,88 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
                             l[j][e] = fmaf(x, MASKED && ((hidden >> (((2 * h + n) * ROW_TILES + j) * 2 + e)) & 1u) ? 0.f : inv[h][n], l[j][e]);
                         }
                 }
-            copies_wait<2 * STAGES - 1>();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t pf[ROW_TILES][2];
-#pragma unroll
-                for (int j = 0; j < ROW_TILES; ++j) {
-                    pf[j][0] = turned(pack(s[h][j][0], s[h][j][1]));
-                    pf[j][1] = turned(pack(s[h][j][2], s[h][j][3]));
-                }
-#pragma unroll
-                for (int u = 0; u < VN; ++u) {
-                    uint32_t v[4][VU / 4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) read_slot<VU>(base + K_BYTES + (((h * 4 + i) * VN + u) * 32 + lane) * VU, v[i]);
-#pragma unroll
-                    for (int k = 0; k < VU / 4; ++k)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {        // two columns of four keys
-                            uint32_t a[4];
-                            halves<STORE>(__byte_perm(v[0][k], v[1][k], x ? 0x7362 : 0x5140), a[0], a[1]);
-                            halves<STORE>(__byte_perm(v[2][k], v[3][k], x ? 0x7362 : 0x5140), a[2], a[3]);
-#pragma unroll
-                            for (int j = 0; j < ROW_TILES; ++j) mma(o[j][u * (VU / 2) + 2 * k + x], a[0], a[1], a[2], a[3], pf[j]);
-                        }
-                }
-            }
         };
 
         int stage = 0;
+#pragma unroll 1
         for (int i = mine_first; i < end; i += WARPS) {
             const int key0 = key_of(i);
             const Pages after = lookup(i + (STAGES + 1) * WARPS);
-            if (key0 > pos_last || (key0 + UNIT <= lo_first && key0 >= c.keep)) {      // the segment's other rows see it
-                copies_wait<2 * STAGES - 2>();
-                fetch_keys(i + STAGES * WARPS, stage, next);
-            } else if (biased) tile(i, stage, std::true_type{}, std::true_type{});
-            else if (key0 + UNIT - 1 <= pos_first && key0 >= lo_last) tile(i, stage, std::false_type{}, std::false_type{});
-            else tile(i, stage, std::true_type{}, std::false_type{});
+            const uint32_t base = slots + stage * STAGE_BYTES;
+            const bool any = key0 <= pos_last && (key0 + UNIT > lo_first || key0 < c.keep);       // else other rows of the segment see it
+            uint32_t kb[2], vb[2];
+            copies_wait<2 * STAGES - 1>();
+            __syncwarp();                                    // all lanes' copies
+            if (any) {
+                uint32_t part[2][2][ROW_TILES][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int j = 0; j < ROW_TILES; ++j) part[h][x][j][0] = part[h][x][j][1] = part[h][x][j][2] = part[h][x][j][3] = 0u;
+                    read_slot<4>(base + 2 * K_BYTES + (8 * h + (g >> 1)) * 4, &kb[h]);
+                    read_slot<4>(base + 2 * K_BYTES + (8 * h + 4 + (g >> 1)) * 4, &vb[h]);
+                }
+#pragma unroll
+                for (int u = 0; u < KN; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t word[2][KU / 4];
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            read_slot<KU>(base + h * 16 * D + 2 * n * D + (D == 128 ? at_lane.k ^ (64 * u) : at_lane.k + 4 * KU * u), word[n]);
+#pragma unroll
+                        for (int k = 0; k < KU / 8; ++k)
+#pragma unroll
+                            for (int j = 0; j < ROW_TILES; ++j)
+#pragma unroll
+                                for (int x = 0; x < 2; ++x)
+                                    mma8<STORE>(part[h][x][j], word[0][2 * k], word[1][2 * k], word[0][2 * k + 1], word[1][2 * k + 1], qf[j][x][u * (KU / 8) + k]);
+                    }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < ROW_TILES; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[h][j][e] = joined<STORE>(part[h][0][j][e], part[h][1][j][e]);
+            }
+            __syncwarp();                                    // all lanes have read the keys: their place is filled anew, STAGES tiles ahead
+            fetch_keys(i + STAGES * WARPS, stage, next);
+            if (any) {
+                if (!biased && key0 + UNIT - 1 <= pos_first && key0 >= lo_last) weigh(key0, kb, vb, std::false_type{});
+                else weigh(key0, kb, vb, std::true_type{});
+            }
+            copies_wait<2 * STAGES - 1>();
+            __syncwarp();
+            if (any) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t pf[ROW_TILES][2];
+#pragma unroll
+                    for (int j = 0; j < ROW_TILES; ++j) {
+                        pf[j][0] = turned(pack(s[h][j][0], s[h][j][1]));
+                        pf[j][1] = turned(pack(s[h][j][2], s[h][j][3]));
+                    }
+#pragma unroll
+                    for (int u = 0; u < VN; ++u) {
+                        uint32_t v[4][VU / 4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) read_slot<VU>(base + K_BYTES + h * 16 * D + (i & 2) * D + at_lane.v[i & 1] + u * 8 * VU, v[i]);
+#pragma unroll
+                        for (int k = 0; k < VU / 4; ++k)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {        // two columns of four keys
+                                uint32_t a[4];
+                                halves<STORE>(__byte_perm(v[0][k], v[1][k], x ? 0x7362 : 0x5140), a[0], a[1]);
+                                halves<STORE>(__byte_perm(v[2][k], v[3][k], x ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+                                for (int j = 0; j < ROW_TILES; ++j) mma(o[j][u * (VU / 2) + 2 * k + x], a[0], a[1], a[2], a[3], pf[j]);
+                            }
+                    }
+                }
+            }
+            __syncwarp();
             fetch_values(i + STAGES * WARPS, stage, next);
             next = after;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -701,14 +734,14 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
 
 template <int STORE, int ROW_TILES>
 static int launch(Params p, int sms, long long pieces, cudaStream_t stream) {
-    const size_t smem = WARPS * WARP_BYTES + (size_t)(p.segments + 1) * 4;
+    const size_t smem = WARPS * warp_bytes<ROW_TILES> + (size_t)(p.segments + 1) * 4;
     static int configured = -1;                              // the device that has been told of the shared memory
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
     if (configured != device) {
         e = cudaFuncSetAttribute(attention_quant_kernel<STORE, ROW_TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 WARPS * WARP_BYTES + (MAX_SEGMENTS + 1) * 4);
+                                 WARPS * warp_bytes<ROW_TILES> + (MAX_SEGMENTS + 1) * 4);
         if (e != cudaSuccess) return (int)e;
         configured = device;
     }
