@@ -13,6 +13,7 @@ using namespace cq;
 // Keys and values are made in float64 from the inputs (a few operations a number, of rows that are few beside the queries): a code
 // is the rounding of the definition's number, whichever kernel writes it, and not of a float32 that lies beside a border.  The scale
 // needs the whole row's largest magnitude before the first code is written.
+constexpr int APPEND_ROWS = 4;
 struct AppendParams {
     const void* qkv;
     int row_stride;
@@ -123,39 +124,56 @@ __global__ void append_quant_any_kernel(const AppendParams p) {
 }
 
 // bfloat16, heads of 8 LANES numbers, rotated halves in steps of eight: LANES lanes hold a head, eight neighbouring numbers each, and a
-// rotation partner is some lanes away.  A block takes a row; its groups of lanes go through the row's heads with the same
-// place in each, so that a row's angles are read once.
-// Bound by bytes in long prompts: 2,048 rows of 36 heads of 128 (34 MB in and out) take APPEND_US, a warp a head with a number a lane 47 us.
+// rotation partner is some lanes away.  A block takes `rows` rows, whose pages and angles it looks up once, and its groups of lanes go through
+// their heads, with three in flight.
+// Bound by the way from a row's position to its angles and by what is in flight: 2,048 rows of 36 heads of 128 (38 MB in and out) take APPEND_US
+// in blocks of four rows, 22 a block a row; a warp a head with a number a lane took 47.
 template <int LANES, int STORE, bool NORM>
-__global__ void __launch_bounds__(256) append_quant_vec_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendParams p, int rows) {
     constexpr int D = 8 * LANES;
-    // The row's metadata, tables and biases are older than the product before this kernel.
-    const int row = blockIdx.x, lane = threadIdx.x & 31, li = lane & (LANES - 1), d = 8 * li;
+    extern __shared__ __align__(16) float angles[];          // [rows][cos, sin][rot_half]
+    __shared__ long long slots[APPEND_ROWS];
+    // The rows' metadata and tables are older than the product before this kernel.
+    const int row0 = blockIdx.x * rows, lane = threadIdx.x & 31, li = lane & (LANES - 1), d = 8 * li, half = p.rot_half;
     const uint32_t group_mask = (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u) << (lane & ~(LANES - 1));
-    const int groups = blockDim.x / LANES, heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0);
-    const int pos = p.positions[row], rot = 2 * p.rot_half;
-    const size_t angle = angles_of(p, pos, threadIdx.x == 0);
-    const long long slot = p.write_kv ? slot_of(p, row, pos, threadIdx.x == 0) : -1;
-    const bool rotated = d < rot, low = d < p.rot_half;
-    const int partner = (lane & ~(LANES - 1)) + (rotated ? (low ? d + p.rot_half : d - p.rot_half) / 8 : li);
-    float cs[8], sn[8];
-    if (rotated) {
-        const size_t t = angle + (low ? d : d - p.rot_half);
-#pragma unroll
-        for (int k = 0; k < 8; k += 4) {
-            const float4 c = *reinterpret_cast<const float4*>(p.cos_t + t + k), s = *reinterpret_cast<const float4*>(p.sin_t + t + k);
-            cs[k] = c.x; cs[k + 1] = c.y; cs[k + 2] = c.z; cs[k + 3] = c.w;
-            sn[k] = low ? -s.x : s.x; sn[k + 1] = low ? -s.y : s.y; sn[k + 2] = low ? -s.z : s.z; sn[k + 3] = low ? -s.w : s.w;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) { cs[k] = 1.f; sn[k] = 0.f; }
+    const int groups = blockDim.x / LANES, heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), rot = 2 * half, here = min(rows, p.T - row0);
+    if ((int)threadIdx.x < here) {
+        const int pos = p.positions[row0 + threadIdx.x];
+        slots[threadIdx.x] = p.write_kv ? slot_of(p, row0 + threadIdx.x, pos, true) : -1;
+        angles_of(p, pos, true);
     }
+    for (int i = 4 * threadIdx.x; i < here * rot; i += 4 * blockDim.x) {
+        const int r = i / rot, at = i - r * rot;
+        const size_t angle = angles_of(p, p.positions[row0 + r], false);
+        *reinterpret_cast<float4*>(angles + i) = *reinterpret_cast<const float4*>(at < half ? p.cos_t + angle + at : p.sin_t + angle + at - half);
+    }
+    const bool rotated = d < rot, low = d < half;
+    const int partner = (lane & ~(LANES - 1)) + (rotated ? (low ? d + half : d - half) / 8 : li);
     pdl_wait();
     pdl_launch_dependents();
-    const bf16* const rows = (const bf16*)p.qkv + (size_t)row * p.row_stride;
-    for (int head = threadIdx.x / LANES; head < heads; head += groups) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(rows + (size_t)head * D + d);
+    __syncthreads();
+    struct Place { int row, head; };
+    auto settle = [&](Place x) { while (x.head >= heads) { x.head -= heads; ++x.row; } return x; };
+    auto load = [&](const Place& x) {
+        return x.row < here ? *reinterpret_cast<const uint4*>((const bf16*)p.qkv + (size_t)(row0 + x.row) * p.row_stride + (size_t)x.head * D + d) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    Place now = settle({0, (int)threadIdx.x / LANES}), then = settle({now.row, now.head + groups}), last = settle({then.row, then.head + groups});
+    uint4 raw = load(now), next = load(then), after = load(last);
+    for (; now.row < here; now = then, then = last, last = settle({last.row, last.head + groups}), raw = next, next = after, after = load(last)) {
+        const int row = row0 + now.row, head = now.head;
+        const long long slot = slots[now.row];
+        float cs[8], sn[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { cs[k] = 1.f; sn[k] = 0.f; }
+        if (rotated) {
+            const float* const at = angles + now.row * rot + (low ? d : d - half);
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                const float4 c = *reinterpret_cast<const float4*>(at + k), s = *reinterpret_cast<const float4*>(at + half + k);
+                cs[k] = c.x; cs[k + 1] = c.y; cs[k + 2] = c.z; cs[k + 3] = c.w;
+                sn[k] = low ? -s.x : s.x; sn[k + 1] = low ? -s.y : s.y; sn[k + 2] = low ? -s.z : s.z; sn[k + 3] = low ? -s.w : s.w;
+            }
+        }
         const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
         float b[8], w[8];
         const bool is_q = head < p.Hq, is_v = head >= p.Hq + p.Hkv;
@@ -234,15 +252,16 @@ __global__ void __launch_bounds__(256) append_quant_vec_kernel(const AppendParam
 
 template <int LANES>
 static int append_vec(const AppendParams& p, int store, cudaStream_t stream) {
-    // A group of lanes a head while rows are few (one row of 18 heads: a pass), half as many groups where rows fill the SMs anyway.
-    const int heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), wanted = (heads * LANES + 31) / 32 * 32;
-    const dim3 grid(p.T), block(wanted < 256 ? wanted : p.T >= 1024 && wanted >= 128 ? 128 : 256);
+    // A group of lanes a head and a block a row while rows are few, four rows a block from there on.
+    const int heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), wanted = (heads * LANES + 31) / 32 * 32, rows = p.T >= 512 ? APPEND_ROWS : 1;
+    const dim3 grid((p.T + rows - 1) / rows), block(wanted < 256 ? wanted : 256);
+    const size_t smem = (size_t)rows * 2 * p.rot_half * sizeof(float);
     if (store == KVB_E4M3) {
-        if (p.eps > 0.f) kvb_launch(append_quant_vec_kernel<LANES, KVB_E4M3, true>, grid, block, 0, stream, p);
-        else kvb_launch(append_quant_vec_kernel<LANES, KVB_E4M3, false>, grid, block, 0, stream, p);
+        if (p.eps > 0.f) kvb_launch(append_quant_vec_kernel<LANES, KVB_E4M3, true>, grid, block, smem, stream, p, rows);
+        else kvb_launch(append_quant_vec_kernel<LANES, KVB_E4M3, false>, grid, block, smem, stream, p, rows);
     } else {
-        if (p.eps > 0.f) kvb_launch(append_quant_vec_kernel<LANES, KVB_INT8, true>, grid, block, 0, stream, p);
-        else kvb_launch(append_quant_vec_kernel<LANES, KVB_INT8, false>, grid, block, 0, stream, p);
+        if (p.eps > 0.f) kvb_launch(append_quant_vec_kernel<LANES, KVB_INT8, true>, grid, block, smem, stream, p, rows);
+        else kvb_launch(append_quant_vec_kernel<LANES, KVB_INT8, false>, grid, block, smem, stream, p, rows);
     }
     return kvb_launch_status();
 }
@@ -288,6 +307,8 @@ KVB_API int kvb_append_quant(int dtype, int store, const void* qkv, int row_stri
 // its blocks: 0 .. kept - 1, then from `first` on (kernels/cache_plan.py).  Block i becomes page i of k_out / v_out [n, Hkv, 64, D], and
 // out_table[segment, block] = i.  Keys that no row of the segment sees (behind its end; before the first row's window, unless among the
 // first `keep`) become zeros, whatever their pages hold.
+// `for_scores`: for a kernel that multiplies weights of zero, too, by values - a token whose key or value is not finite then gets a key of NaN,
+// which no row meets that does not see the token, and a value of zeros.
 constexpr int READ_BLOCK = 64;
 struct ExpandParams {
     const uint8_t* k_codes;
@@ -305,9 +326,16 @@ struct ExpandParams {
     void* k_out;
     void* v_out;
     int* out_table;
-    int out_stride, Hkv, D;
+    int out_stride, Hkv, D, for_scores;
     int* err;
 };
+// What multiplies the codes of the pool's row `at`.
+__device__ __forceinline__ float read_scale(const ExpandParams& p, bool values, long long at) {
+    const int byte = (values ? p.v_scales : p.k_scales)[at];
+    if (!p.for_scores) return scale_up(byte);
+    const bool broken = byte == NOT_FINITE || (values ? p.k_scales : p.v_scales)[at] == NOT_FINITE;
+    return broken ? (values ? 0.f : __int_as_float(0x7fffffff)) : scale_up(byte);
+}
 
 // The segment that block i belongs to, and which of its blocks it is.
 __device__ __forceinline__ void find_block(const ExpandParams& p, int i, int& seg, int& block) {
@@ -329,7 +357,6 @@ __global__ void expand_any_kernel(const ExpandParams p) {
     const int kv_len = p.seg_kv_len[seg], lo = first_seen_key(kv_len - p.seg_q_len[seg], p.reach), keep = p.reach > 0 ? p.keep : 0;
     if (hk == 0 && !values && threadIdx.x == 0 && block < p.out_stride) p.out_table[(size_t)seg * p.out_stride + block] = i;
     const uint8_t* codes = values ? p.v_codes : p.k_codes;
-    const uint8_t* scales = values ? p.v_scales : p.k_scales;
     T* out = (T*)(values ? p.v_out : p.k_out) + ((size_t)i * p.Hkv + hk) * READ_BLOCK * D;
     const int lane = threadIdx.x & 31;
     for (int r = threadIdx.x >> 5; r < READ_BLOCK; r += blockDim.x >> 5) {
@@ -341,7 +368,7 @@ __global__ void expand_any_kernel(const ExpandParams p) {
             if (page >= 0 && page < p.num_pages) at = ((long long)page * p.Hkv + hk) * p.page_size + key % p.page_size;
             else if (lane == 0) atomicOr(p.err, KVB_DEV_BAD_PAGE);
         }
-        const float up = at >= 0 ? scale_up(scales[at]) : 0.f;
+        const float up = at >= 0 ? read_scale(p, values, at) : 0.f;
         for (int d = lane; d < D; d += 32)
             out[(size_t)r * D + d] = from_f32<T>(at >= 0 ? code_value<STORE>(codes[at * D + d]) * up : 0.f);
     }
@@ -372,14 +399,13 @@ __global__ void __launch_bounds__(256) expand_vec_kernel(const ExpandParams p) {
     const int kv_len = p.seg_kv_len[seg], lo = first_seen_key(kv_len - p.seg_q_len[seg], p.reach), keep = p.reach > 0 ? p.keep : 0;
     const int* const table = p.block_table + (size_t)seg * p.table_stride;
     const uint8_t* const codes = values ? p.v_codes : p.k_codes;
-    const uint8_t* const scales = values ? p.v_scales : p.k_scales;
     T* const out = (T*)(values ? p.v_out : p.k_out) + ((size_t)i * p.Hkv + hk) * READ_BLOCK * D;
     constexpr int FLIGHT = 4;
     bool waited = false;
     for (int c0 = threadIdx.x; c0 < READ_BLOCK * chunks; c0 += FLIGHT * 256) {
         long long at[FLIGHT];
         uint2 code[FLIGHT];
-        int byte[FLIGHT];
+        float up[FLIGHT];
 #pragma unroll
         for (int f = 0; f < FLIGHT; ++f) {
             const int c = c0 + f * 256, r = c / chunks, key = block * READ_BLOCK + r;
@@ -400,20 +426,19 @@ __global__ void __launch_bounds__(256) expand_vec_kernel(const ExpandParams p) {
 #pragma unroll
         for (int f = 0; f < FLIGHT; ++f) {
             code[f] = make_uint2(0u, 0u);
-            byte[f] = 0;
+            up[f] = 0.f;
             if (at[f] >= 0) {
                 code[f] = *reinterpret_cast<const uint2*>(codes + at[f] * D + ((c0 + f * 256) % chunks) * 8);
-                byte[f] = scales[at[f]];
+                up[f] = read_scale(p, values, at[f]);
             }
         }
 #pragma unroll
         for (int f = 0; f < FLIGHT; ++f) {
             const int c = c0 + f * 256;
             if (c >= READ_BLOCK * chunks) break;
-            const float up = at[f] >= 0 ? scale_up(byte[f]) : 0.f;
             float x[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = code_value<STORE>(((k < 4 ? code[f].x : code[f].y) >> (8 * (k & 3))) & 255u) * up;
+            for (int k = 0; k < 8; ++k) x[k] = code_value<STORE>(((k < 4 ? code[f].x : code[f].y) >> (8 * (k & 3))) & 255u) * up[f];
             store8<T>(out + (size_t)c * 8, x);
         }
     }
@@ -431,12 +456,12 @@ static int expand(const ExpandParams& p, int store, int n, cudaStream_t stream) 
 KVB_API int kvb_cache_expand(int dtype, int store, const void* k_codes, const void* v_codes, const void* k_scales, const void* v_scales, int num_pages,
                              const int* block_table, int table_stride, int page_size, const int* ranges, int segments, int n,
                              const int* seg_q_len, const int* seg_kv_len, int reach, int keep, void* k_out, void* v_out, int* out_table, int out_stride, int Hkv, int D,
-                             int* err, cudaStream_t stream) {
+                             int for_scores, int* err, cudaStream_t stream) {
     if (n <= 0) return KVB_OK;
     if (store != KVB_E4M3 && store != KVB_INT8) return KVB_ERR_DTYPE;
     if (D < 1 || Hkv < 1 || Hkv > 65535 || page_size < 1 || num_pages < 1 || keep < 0 || segments < 1) return KVB_ERR_SHAPE;
     const ExpandParams p = {(const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scales, (const uint8_t*)v_scales, num_pages, block_table,
-                            table_stride, page_size, ranges, segments, seg_q_len, seg_kv_len, reach, keep, k_out, v_out, out_table, out_stride, Hkv, D, err};
+                            table_stride, page_size, ranges, segments, seg_q_len, seg_kv_len, reach, keep, k_out, v_out, out_table, out_stride, Hkv, D, for_scores, err};
     if (dtype == KVB_BF16) return expand<bf16>(p, store, n, stream);
     if (dtype == KVB_F32) return expand<float>(p, store, n, stream);
     return KVB_ERR_DTYPE;

@@ -182,8 +182,8 @@ _SIGNATURES = {
                              _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int,
                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
         "kvb_cache_expand": [_c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int,
-                             _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p,
-                             _c_void_p],
+                             _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                             _c_void_p, _c_void_p],
         "kvb_attention_quant_any": [_c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p,
                                     _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_float,
                                     _c_float, _c_void_p, _c_void_p],
@@ -945,18 +945,23 @@ class CudaKernels(KernelSet):
                 return plan, singles
         return None, False
 
-    def expand_cache(self, batch: StepBatch, kv: PagedKVView, dtype: torch.dtype, workspace, reach: Optional[int] = None) -> PagedKVView:
+    def expand_cache(self, batch: StepBatch, kv: PagedKVView, dtype: torch.dtype, workspace, reach: Optional[int] = None,
+                     portions: bool = False, for_attention: bool = False) -> PagedKVView:
         """The keys and values that a step's rows see in a cache entry in eight bits, as float32 or bfloat16 (which holds them
         exactly) in pages of 64 tokens that `paged_attention` takes: one page for every 64 keys of every request of the plan (see
-        `cache_expand_planner`), in order.  Keys behind a request's last, and before its rows' window, are zeros.  The pages lie in
-        the workspace and last until its next call."""
+        `cache_expand_planner`) - with `portions`, of every request that brings more than one token - in order.  Keys behind a request's last,
+        and before its rows' window, are zeros.  `for_attention`: a token whose key or value is not finite has a key of NaN and a value
+        of zeros, so that rows which do not see it are none the worse.  The pages lie in the workspace and last until its next call."""
         spec = kv.spec
         reach = spec.reach if reach is None else int(reach)
         store = self._quantised_entry(kv, "expand_cache")
-        plan, _ = self._expand_plan(batch, reach, spec.keep_first)
-        if plan is None:
+        plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
+        if plan is None or not (portions or with_singles):
             raise KernelError("expand_cache: the step has no list of blocks (cache_expand_planner)")
-        n, S, D, Hkv = plan.counts["blocks"], batch.num_segments, spec.head_dim, spec.num_kv_heads
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise KernelError(f"expand_cache: rows are read back as float32 or bfloat16, not {dtype}")
+        n, ranges = (plan.counts["portion_blocks"], plan.arrays["portions"]) if portions else (plan.counts["blocks"], plan.arrays["ranges"])
+        S, D, Hkv = batch.num_segments, spec.head_dim, spec.num_kv_heads
         name = "f32" if dtype == torch.float32 else "bf16"
         k_out = workspace.buffer(f"cache.expand_k_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
         v_out = workspace.buffer(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
@@ -967,15 +972,18 @@ class CudaKernels(KernelSet):
             self._count("cache_expand")
             _check(self._cache_quant.kvb_cache_expand(
                 _dtype_code(dtype), store, _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
-                _ptr(kv.block_table), kv.block_table.shape[1], kv.page_size, _ptr(plan.arrays["ranges"]), S, n, _ptr(batch.seg_q_len),
-                _ptr(batch.seg_kv_len), reach, spec.keep_first, _ptr(k_out), _ptr(v_out), _ptr(table), stride, Hkv, D, _ptr(self.error_word),
+                _ptr(kv.block_table), kv.block_table.shape[1], kv.page_size, _ptr(ranges), S, n, _ptr(batch.seg_q_len),
+                _ptr(batch.seg_kv_len), reach, spec.keep_first, _ptr(k_out), _ptr(v_out), _ptr(table), stride, Hkv, D, int(for_attention), _ptr(self.error_word),
                 self._stream()), "expand_cache")
         return view
 
     QUANT_MAX_SEGMENTS = 4096
     # Bytes of keys and values that a layer reads back for a step's portions; longer ones read the codes in place.
     CACHE_EXPAND_MAX_BYTES = 1 << 30
-    quant_expand_min_rows = 64           # portions of at least this many tokens have their keys and values read back first
+    # Portions have their keys and values read back first from this many tokens on, and where they have no more than this many blocks of 64
+    # keys each on average.  Codes in place and read back, us, 28 heads of 128 (4 of keys): 16 rows behind none 10 and 7, behind 2,000 18 and 22,
+    # behind 16,000 42 and 107; 64 rows 14 and 9, 33 and 39, 119 and 138; 128 rows 24 and 11, 48 and 26, 217 and 79.
+    quant_expand_min_rows, quant_expand_max_blocks = 128, 16
     quant_min_units = 8                  # units of 32 keys a block of csrc/attention_quant.cu takes at least
 
     def _quant_library(self, head_dim: int) -> Tuple[_Library, int, int]:
@@ -1004,15 +1012,17 @@ class CudaKernels(KernelSet):
                   and (kv.k_scales.data_ptr() | kv.v_scales.data_ptr()) % 4 == 0)
         # Read back first: portions of enough rows, and what the codes' own kernel does not take.
         expand = False
-        if not direct or (batch.max_q_len >= self.quant_expand_min_rows and group <= 16):
+        if not direct or (batch.max_q_len > 1 and group <= 16):
             plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
             paged = batch.plans.get(PagedAttentionPlanner.name)
             singles = S if batch.max_q_len == 1 or paged is None else paged.counts["decode_items"]
-            expand = (plan is not None and plan.counts["blocks"] > 0 and paged is not None and workspace is not None
-                      and 4 * plan.counts["blocks"] * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES
-                      and (direct or with_singles or singles == 0))
+            portions_only = direct or not with_singles
+            blocks = 0 if plan is None else plan.counts["portion_blocks" if portions_only else "blocks"]
+            expand = (blocks > 0 and paged is not None and workspace is not None and (direct or with_singles or singles == 0)
+                      and 2 * q.element_size() * blocks * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES
+                      and (not direct or batch.max_q_len >= self.quant_expand_min_rows or blocks <= self.quant_expand_max_blocks * (S - singles)))
         if expand:
-            view = self.expand_cache(batch, kv, q.dtype, workspace, reach)
+            view = self.expand_cache(batch, kv, q.dtype, workspace, reach, portions_only, for_attention=True)
             portions = batch
             if direct and singles:           # single tokens keep to their codes: the portions' kernels leave them out
                 portions = dataclasses.replace(batch, plans={**batch.plans, PagedAttentionPlanner.name: StepPlan(

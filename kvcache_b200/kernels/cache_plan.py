@@ -8,7 +8,7 @@ from typing import Dict, Tuple
 
 import numpy as np
 
-from ..parts.base import StepPlanner, first_seen
+from ..parts.base import StepPlanner
 
 EXPAND_BLOCK = 64                # keys of a block that is read back, and tokens of the pages they become
 
@@ -16,8 +16,8 @@ EXPAND_BLOCK = 64                # keys of a block that is read back, and tokens
 class CacheExpandPlanner(StepPlanner):
     """`ranges`: [segments + 1, 3] - how many blocks the segments before this one bring, and which its own are: blocks 0 .. kept - 1 (the
     first keys that a window keeps), then those from `first` up to its last key's.  The last row holds the total alone.
-
-    `singles` False: segments of one token bring none, so that a step of decoded tokens has the same counts whatever its lengths."""
+    `portions`: the same where segments of one token bring none (their attention reads the codes); without `singles` the only list, so that a
+    step of decoded tokens has the same counts whatever its lengths."""
 
     def __init__(self, reach: int = 0, keep_first: int = 0, singles: bool = True):
         self.reach, self.keep_first, self.singles = reach, keep_first, singles
@@ -28,18 +28,29 @@ class CacheExpandPlanner(StepPlanner):
         return f"cache_expand.r{reach}.k{keep_first}" + ("" if singles else ".portions")
 
     def sections(self, num_tokens: int, num_segments: int) -> Dict[str, int]:
-        return {"ranges": 3 * (num_segments + 1)}
+        words = 3 * (num_segments + 1)
+        return {"ranges": words, "portions": words} if self.singles else {"portions": words}
+
+    def _ranges(self, starts, counts, least: int) -> np.ndarray:
+        starts, counts = np.asarray(starts, dtype=np.int64), np.asarray(counts, dtype=np.int64)
+        if self.reach > 0:
+            lo = np.maximum(0, starts - self.reach + 1)
+        elif self.reach < 0:
+            lo = starts - starts % -self.reach
+        else:
+            lo = np.zeros_like(starts)
+        first = lo // EXPAND_BLOCK
+        kept = np.minimum(-(-self.keep_first // EXPAND_BLOCK), first) if self.reach > 0 else np.zeros_like(first)
+        blocks = np.where(counts >= least, kept + -(-(starts + counts) // EXPAND_BLOCK) - first, 0)
+        ranges = np.zeros((len(counts) + 1, 3), dtype=np.int32)
+        np.cumsum(blocks, out=ranges[1:, 0])
+        ranges[:-1, 1], ranges[:-1, 2] = kept, first
+        return ranges
 
     def plan(self, starts, counts) -> Tuple[Dict[str, np.ndarray], Dict[str, int]]:
-        ranges = np.zeros((len(counts) + 1, 3), dtype=np.int32)
-        total = 0
-        for i, (start, count) in enumerate(zip(starts, counts)):
-            ranges[i, 0] = total
-            if count < 1 or (count == 1 and not self.singles):
-                continue
-            first = first_seen(int(start), self.reach) // EXPAND_BLOCK
-            kept = min(-(-self.keep_first // EXPAND_BLOCK), first) if self.reach > 0 else 0
-            ranges[i, 1:] = kept, first
-            total += kept + -(-(int(start) + int(count)) // EXPAND_BLOCK) - first
-        ranges[-1, 0] = total
-        return {"ranges": ranges.reshape(-1)}, {"blocks": total}
+        portions = self._ranges(starts, counts, 2)
+        arrays, numbers = {"portions": portions.reshape(-1)}, {"portion_blocks": int(portions[-1, 0])}
+        if self.singles:
+            ranges = self._ranges(starts, counts, 1)
+            arrays["ranges"], numbers["blocks"] = ranges.reshape(-1), int(ranges[-1, 0])
+        return arrays, numbers

@@ -45,8 +45,13 @@ def test_lists_of_blocks(reach, keep, singles):
     planner = CacheExpandPlanner(reach, keep if reach > 0 else 0, singles)
     starts, counts = [0, 0, 63, 64, 500, 1000, 17], [1, 64, 1, 2, 130, 1, 300]
     arrays, numbers = planner.plan(np.asarray(starts), np.asarray(counts))
-    ranges = arrays["ranges"].reshape(-1, 3)
-    assert len(arrays["ranges"]) <= planner.sections(sum(counts), len(counts))["ranges"]
+    assert set(arrays) == ({"ranges", "portions"} if singles else {"portions"})
+    assert all(len(a) <= planner.sections(sum(counts), len(counts))[name] for name, a in arrays.items())
+    for name, total in (("ranges", "blocks"), ("portions", "portion_blocks")) if singles else (("portions", "portion_blocks"),):
+        check_ranges(arrays[name].reshape(-1, 3), numbers[total], starts, counts, reach, keep, name == "ranges")
+
+
+def check_ranges(ranges, total, starts, counts, reach, keep, singles):
     at = 0
     for i, (start, count) in enumerate(zip(starts, counts)):
         assert ranges[i, 0] == at
@@ -60,12 +65,12 @@ def test_lists_of_blocks(reach, keep, singles):
         else:
             assert not blocks
         at += end
-    assert numbers["blocks"] == at == ranges[-1, 0]
+    assert total == at == ranges[-1, 0]
 
 
 def test_steps_of_single_tokens_have_one_plan():
     planner = CacheExpandPlanner(0, 0, False)
-    assert planner.plan([5, 900], [1, 1])[1] == planner.plan([70, 3], [1, 1])[1] == {"blocks": 0}
+    assert planner.plan([5, 900], [1, 1])[1] == planner.plan([70, 3], [1, 1])[1] == {"portion_blocks": 0}
 
 
 def _bare():
