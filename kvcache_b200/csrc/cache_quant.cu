@@ -13,7 +13,7 @@ using namespace cq;
 // Keys and values are made in float64 from the inputs (a few operations a number, of rows that are few beside the queries): a code
 // is the rounding of the definition's number, whichever kernel writes it, and not of a float32 that lies beside a border.  The scale
 // needs the whole row's largest magnitude before the first code is written.
-constexpr int APPEND_ROWS = 4;
+constexpr int APPEND_ROWS = 16;        // rows a block takes at most
 struct AppendParams {
     const void* qkv;
     int row_stride;
@@ -119,7 +119,7 @@ __global__ void append_quant_any_kernel(const AppendParams p) {
     const float down = scale_down(byte);
     const long long at = slot + (long long)(is_v ? head - p.Hq - p.Hkv : head - p.Hq) * p.page_size;
     uint8_t* codes = (is_v ? p.v_codes : p.k_codes) + at * D;
-    for (int d = lane; d < D; d += 32) codes[d] = (uint8_t)code_of<STORE>(h.at(d), down);
+    for (int d = lane; d < D; d += 32) codes[d] = down != 0.f ? (uint8_t)code_of<STORE>(h.at(d), down) : (uint8_t)0;
     if (lane == 0) (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)byte;
 }
 
@@ -242,8 +242,9 @@ __global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendPa
         const int byte = scale_byte<STORE>(top);
         const float down = scale_down(byte);
         uint32_t codes[2] = {0u, 0u};
+        if (down != 0.f)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) codes[k >> 2] |= code_of<STORE>(x[k], down) << (8 * (k & 3));
+            for (int k = 0; k < 8; ++k) codes[k >> 2] |= code_of<STORE>(x[k], down) << (8 * (k & 3));
         const long long at = slot + (long long)(is_v ? head - p.Hq - p.Hkv : head - p.Hq) * p.page_size;
         *reinterpret_cast<uint2*>((is_v ? p.v_codes : p.k_codes) + at * D + d) = make_uint2(codes[0], codes[1]);
         if (li == 0) (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)byte;
@@ -252,8 +253,10 @@ __global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendPa
 
 template <int LANES>
 static int append_vec(const AppendParams& p, int store, cudaStream_t stream) {
-    // A group of lanes a head and a block a row while rows are few, four rows a block from there on.
-    const int heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), wanted = (heads * LANES + 31) / 32 * 32, rows = p.T >= 512 ? APPEND_ROWS : 1;
+    // A group of lanes a head; a block a row, or as many rows as leave no more blocks than the SMs hold at once (three each: with four rows a
+    // block 2,048 rows were 512 blocks and took 24 us).
+    const int heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), wanted = (heads * LANES + 31) / 32 * 32, at_once = 3 * kvb_sm_count();
+    const int rows = (p.T + at_once - 1) / at_once < APPEND_ROWS ? (p.T + at_once - 1) / at_once : APPEND_ROWS;
     const dim3 grid((p.T + rows - 1) / rows), block(wanted < 256 ? wanted : 256);
     const size_t smem = (size_t)rows * 2 * p.rot_half * sizeof(float);
     if (store == KVB_E4M3) {

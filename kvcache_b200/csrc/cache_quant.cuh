@@ -34,14 +34,17 @@ __device__ __forceinline__ int scale_byte(uint32_t top) {
 __device__ __forceinline__ float scale_down(int byte) { return byte == NOT_FINITE ? 0.f : __int_as_float((2 * BIAS - byte) << 23); }
 __device__ __forceinline__ float scale_up(int byte) { return __int_as_float(byte == NOT_FINITE ? 0x7fffffff : byte << 23); }
 
-// The code of x 2^-e, in the low byte, rounded once: on the way to e4m3 a float32 that keeps a last bit of what it leaves out.
+// The code of a finite x times 2^-e, in the low byte, rounded once: on the way to e4m3 a float32 whose last bit says that something was left out.
 template <int STORE>
 __device__ __forceinline__ uint32_t code_of(double x, float down) {
-    if (down == 0.f) return 0u;                       // x may be an infinity or NaN
     const double y = x * (double)down;
-    if (STORE == KVB_INT8) return (uint32_t)min(127, max(-127, __double2int_rn(y))) & 0xffu;
-    const float f = __double2float_rz(y);
-    return (uint32_t)__nv_cvt_float_to_fp8((double)f == y ? f : __uint_as_float(__float_as_uint(f) | 1u), __NV_SATFINITE, __NV_E4M3);
+    if (STORE == KVB_INT8) {
+        // Whole numbers by the sum with 1.5 * 2^52; |y| is far below 2^31 but for rows beyond 2^EXP_MAX, which saturate.
+        const int c = __double2loint(fmin(fmax(y, -127.0), 127.0) + 6755399441055744.0);
+        return (uint32_t)c & 0xffu;
+    }
+    const uint32_t left = (__double2loint(y) & 0x1fffffff) != 0 ? 1u : 0u;         // the 29 bits that a float32 has not
+    return (uint32_t)__nv_cvt_float_to_fp8(__uint_as_float(__float_as_uint(__double2float_rz(y)) | left), __NV_SATFINITE, __NV_E4M3);
 }
 template <int STORE>
 __device__ __forceinline__ float code_value(uint32_t code) {
