@@ -15,7 +15,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
-from ..parts.base import PagedKVSpec, PagedKVView, TORCH_DTYPES
+from ..parts.base import STORE_DTYPES, PagedKVSpec, PagedKVView, TORCH_DTYPES
 from ..parts.model import CacheEntry
 from .pages import GroupPages, OutOfPages, pages_for
 from .slots import SlotAllocator
@@ -28,6 +28,8 @@ class CacheGroup:
     pages: GroupPages
     k_pool: Optional[torch.Tensor] = None     # [entries, pages, kv_heads, page_size, head_dim]
     v_pool: Optional[torch.Tensor] = None
+    k_scales: Optional[torch.Tensor] = None   # with `spec.store`: scale bytes, uint8 [entries, pages, kv_heads, page_size]
+    v_scales: Optional[torch.Tensor] = None
 
 
 class CacheManager:
@@ -67,8 +69,15 @@ class CacheManager:
         if self.device is not None:
             for group in self.groups:
                 shape = (len(group.cache_ids), num_pages, group.spec.num_kv_heads, page_size, group.spec.head_dim)
-                group.k_pool = torch.zeros(shape, dtype=self.dtype, device=self.device)
-                group.v_pool = torch.zeros(shape[:-1] + (group.spec.v_head_dim,), dtype=self.dtype, device=self.device)
+                dtype = self._pool_dtype(group.spec)
+                group.k_pool = torch.zeros(shape, dtype=dtype, device=self.device)
+                group.v_pool = torch.zeros(shape[:-1] + (group.spec.v_head_dim,), dtype=dtype, device=self.device)
+                if group.spec.store is not None:
+                    group.k_scales = torch.zeros(shape[:-1], dtype=torch.uint8, device=self.device)
+                    group.v_scales = torch.zeros(shape[:-1], dtype=torch.uint8, device=self.device)
+
+    def _pool_dtype(self, spec: PagedKVSpec) -> torch.dtype:
+        return self.dtype if spec.store is None else STORE_DTYPES[spec.store]
 
     # ---- requests ----------------------------------------------------------
     def admit(self) -> int:
@@ -160,8 +169,10 @@ class CacheManager:
 
     def kv_bytes_per_token(self) -> int:
         """Bytes of keys and values one token adds over all cache entries."""
-        size = torch.empty((), dtype=self.dtype).element_size()
-        return sum(len(g.cache_ids) * g.spec.num_kv_heads * (g.spec.head_dim + g.spec.v_head_dim) * size for g in self.groups)
+        def row(spec: PagedKVSpec) -> int:                   # of one token and head: keys and values, and their scale bytes
+            numbers = spec.head_dim + spec.v_head_dim
+            return numbers * torch.empty((), dtype=self.dtype).element_size() if spec.store is None else numbers + 2
+        return sum(len(g.cache_ids) * g.spec.num_kv_heads * row(g.spec) for g in self.groups)
 
     # ---- views for a step --------------------------------------------------
     def table_rows(self, group: int, slots: Sequence[int]) -> np.ndarray:
@@ -185,8 +196,9 @@ class StepCacheView:
             return None
         g, i = where
         group = self.manager.groups[g]
+        scales = {} if group.k_scales is None else {"k_scales": group.k_scales[i], "v_scales": group.v_scales[i]}
         return PagedKVView(spec=group.spec, k_pages=group.k_pool[i], v_pages=group.v_pool[i],
-                           block_table=self.device_tables[g], page_size=self.manager.page_size, writes=writes)
+                           block_table=self.device_tables[g], page_size=self.manager.page_size, writes=writes, **scales)
 
     def state(self, cache_id: int) -> Optional[torch.Tensor]:
         return self.manager.states.get(cache_id)

@@ -20,6 +20,8 @@ def main(argv=None) -> int:
     parser.add_argument("dir", nargs="?", default="data/qwen05b", help="model folder (config.json, model.safetensors)")
     parser.add_argument("max_new", nargs="?", type=int, default=32)
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    parser.add_argument("--cache-dtype", default="auto", choices=["auto", "e4m3", "int8"],
+                        help="what cached keys and values are held as: the compute type, or eight bits a number")
     parser.add_argument("--temperature", type=float, default=0.0)
     parser.add_argument("--seed", type=int, default=0)
     parser.add_argument("--block-size", type=int, default=16, help="tokens per cache page (reference: BLOCK = 16)")
@@ -41,7 +43,7 @@ def main(argv=None) -> int:
     from ..engine.llm import LLM
     from ..sampling.params import SamplingParams
     total = len(prompt) + args.max_new + 4          # the reference's private pool: P + max_new + 4 (qwen_infer.cu:73-76)
-    llm = LLM(args.dir, EngineOptions(dtype=args.dtype, page_size=args.block_size, max_cached_tokens=total + args.block_size,
+    llm = LLM(args.dir, EngineOptions(dtype=args.dtype, cache_dtype=args.cache_dtype, page_size=args.block_size, max_cached_tokens=total + args.block_size,
                                       max_running=1, max_tokens_per_step=max(len(prompt), 1), chunk_size=max(len(prompt), 1),
                                       use_graphs=args.graph, seed=args.seed))
     params = SamplingParams(max_new_tokens=args.max_new, temperature=args.temperature, seed=args.seed, ignore_eos=True)

@@ -34,6 +34,8 @@ def main(argv=None) -> int:
     parser = argparse.ArgumentParser(prog="qwen_serve", description="continuous batching over token ids")
     parser.add_argument("dir", nargs="?", default="data/qwen05b")
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    parser.add_argument("--cache-dtype", default="auto", choices=["auto", "e4m3", "int8"],
+                        help="what cached keys and values are held as: the compute type, or eight bits a number")
     parser.add_argument("--max-batch", type=int, default=8)
     parser.add_argument("--num-blocks", type=int, default=512)
     parser.add_argument("--block-size", type=int, default=16)
@@ -61,7 +63,7 @@ def main(argv=None) -> int:
     from ..engine.llm import LLM
     from ..engine.scheduler import RequestRejected
     from ..sampling.params import SamplingParams
-    llm = LLM(args.dir, EngineOptions(dtype=args.dtype, page_size=args.block_size, num_pages=args.num_blocks,
+    llm = LLM(args.dir, EngineOptions(dtype=args.dtype, cache_dtype=args.cache_dtype, page_size=args.block_size, num_pages=args.num_blocks,
                                       max_running=args.max_batch, max_tokens_per_step=args.max_tokens_per_step,
                                       chunk_size=args.chunk_size, admission=args.admission, use_graphs=args.graph,
                                       seed=args.seed))

@@ -27,6 +27,8 @@ def main(argv=None) -> int:
     parser = argparse.ArgumentParser(prog="trace_run", description=__doc__.split("\n\n")[0])
     parser.add_argument("--model", required=True, help="folder with config.json and model.safetensors")
     parser.add_argument("--dtype", required=True, choices=["bfloat16", "float32"])
+    parser.add_argument("--cache-dtype", default="auto", choices=["auto", "e4m3", "int8"],
+                        help="what cached keys and values are held as: the compute type, or eight bits a number")
     parser.add_argument("--out", required=True, help="folder for <step>.f32 files")
     parser.add_argument("--max-tokens", type=int, required=True,
                         help="most tokens that live requests hold at any time (each rounded up to 64)")
@@ -43,7 +45,7 @@ def main(argv=None) -> int:
     os.makedirs(args.out, exist_ok=True)
     unit = max(64, args.page_size)                       # a request's tokens are rounded up to this
     capacity = max(unit, (args.max_tokens + unit - 1) // unit * unit)
-    options = EngineOptions(dtype=args.dtype, page_size=args.page_size, max_cached_tokens=capacity,
+    options = EngineOptions(dtype=args.dtype, cache_dtype=args.cache_dtype, page_size=args.page_size, max_cached_tokens=capacity,
                             max_running=args.max_live, max_tokens_per_step=capacity, use_graphs=False)
     core = EngineCore(args.model, options)
     slots: Dict[str, int] = {}

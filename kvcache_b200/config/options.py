@@ -16,9 +16,13 @@ def canonical_dtype(name: str) -> str:
         raise ValueError(f"dtype must be one of bfloat16, float32; got '{name}'") from None
 
 
+CACHE_DTYPES = ("auto", "e4m3", "int8")
+
+
 @dataclass
 class EngineOptions:
     dtype: str = "bfloat16"
+    cache_dtype: str = "auto"              # what cached keys and values are held as: "auto" (`dtype`), "e4m3" or "int8" (eight bits a number)
     page_size: int = 16                    # tokens in a page of the cache
     num_pages: Optional[int] = None        # pages of each cache group; None: from max_cached_tokens
     max_cached_tokens: Optional[int] = None  # pool capacity in tokens when num_pages is None
@@ -34,6 +38,8 @@ class EngineOptions:
 
     def __post_init__(self) -> None:
         self.dtype = canonical_dtype(self.dtype)
+        if self.cache_dtype not in CACHE_DTYPES:
+            raise ValueError(f"cache_dtype must be one of {', '.join(CACHE_DTYPES)}, got '{self.cache_dtype}'")
         if self.page_size < 1 or (self.page_size & (self.page_size - 1)) != 0:
             raise ValueError(f"page_size must be a power of two, got {self.page_size}")
         if self.admission not in ("reserve", "optimistic"):

@@ -39,6 +39,8 @@ class EngineCore:
         max_len = min(max_len, num_pages * options.page_size) if max_len else num_pages * options.page_size
         self.max_model_len = max_len
         self.model = load_model(folder, options.dtype, self.device, max_positions=max_len, strict=options.strict_weights)
+        if options.cache_dtype != "auto":
+            self.model.store_cache(options.cache_dtype)
         self.cache = CacheManager(self.model.cache_entries(), page_size=options.page_size, num_pages=num_pages,
                                   max_slots=options.max_running, max_tokens_per_request=max_len,
                                   dtype=options.dtype, device=self.device)

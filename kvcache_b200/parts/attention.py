@@ -12,7 +12,7 @@ from typing import Dict, Mapping, Optional, Sequence
 import torch
 
 from ..weights.loader import TensorSpec
-from .base import TORCH_DTYPES, BiasedDelta, LayerContext, Mixer, PagedKVSpec, PositionEncoding, reach_code
+from .base import STORE_DTYPES, TORCH_DTYPES, BiasedDelta, LayerContext, Mixer, PagedKVSpec, PositionEncoding, reach_code
 from .position import interleaved_order
 
 
@@ -120,6 +120,7 @@ class GQAAttention(Mixer):
         if (pad_values and dtype == "bfloat16" and self.value_dim < head_dim <= 128 and head_dim % 16 == 0
                 and num_heads // num_kv_heads <= 16):
             self.value_store = head_dim
+        self.cache_store: Optional[str] = None               # see `store_cache`
         self.w_qkv: Optional[torch.Tensor] = None
         self.b_qkv: Optional[torch.Tensor] = None
         self.w_o: Optional[torch.Tensor] = None
@@ -247,15 +248,33 @@ class GQAAttention(Mixer):
         if not self.own_kv:
             return None
         return PagedKVSpec(self.num_kv_heads, self.key_store, self.cache_window,
-                           None if self.value_store == self.key_store else self.value_store, self.keep_first, self.cache_chunk)
+                           None if self.value_store == self.key_store else self.value_store, self.keep_first, self.cache_chunk,
+                           self.cache_store)
+
+    def store_cache(self, store: str) -> None:
+        if store not in STORE_DTYPES:
+            raise ValueError(f"a cache is held as one of {', '.join(STORE_DTYPES)}, not '{store}'")
+        missing = [name for name, there in (("values of another size than keys", self.value_store != self.key_store or self.value_dim != self.head_dim),
+                                            ("keys wider than their numbers", self.key_store != self.head_dim),
+                                            ("norms over whole projections", self.qk_norm_eps is not None and self.qk_norm_scope != "head"),
+                                            ("norms after the rotation", self.qk_norm_eps is not None and self.qk_norm_after_rotation),
+                                            ("blended values", self.value_mix is not None), ("a query temperature", self.q_temperature is not None)) if there]
+        if missing:
+            raise ValueError(", ".join(missing))
+        self.cache_store = store
 
     def step_planners(self, kernels):
         planner = getattr(kernels, "paged_attention_planner", None)
-        return () if planner is None else (planner(),)
+        if planner is None:
+            return ()
+        if self.cache_store is None or not hasattr(kernels, "cache_expand_planner"):
+            return (planner(),)
+        # Portions may have their keys and values read back; single tokens read the codes, so a step of them has one plan.
+        return planner(), kernels.cache_expand_planner(self.reach, self.keep_first, singles=False)
 
     def supports_fold(self, norm, kernels, num_rows: int) -> bool:
         can = getattr(kernels, "can_fold", None)
-        return (self.plain and can is not None and norm.fold_params() is not None
+        return (self.plain and self.cache_store is None and can is not None and norm.fold_params() is not None
                 and can(self.dtype, num_rows, self.hidden, self.q_size + 2 * self.kv_size)
                 and can(self.dtype, num_rows, self.q_size, self.hidden) and self._pair_rows(kernels))
 

@@ -133,6 +133,17 @@ class DecoderModel:
             entries.append(CacheEntry(None, part.state_spec()))
         return entries
 
+    def store_cache(self, store: str) -> None:
+        """Cached keys and values in eight bits ("e4m3", "int8"); raises if a layer's mixer keeps pages that cannot be held so."""
+        problems = []
+        for i, block in enumerate(self.blocks):
+            try:
+                block.mixer.store_cache(store)
+            except ValueError as exc:
+                problems.append(f"layer {i}: {exc}")
+        if problems:
+            raise ValueError(f"a cache held as {store} is not built for this model: " + "; ".join(problems))
+
     def step_planners(self, kernels: Any) -> List[Any]:
         """The planners of all mixers' kernels, each once (by name), in the order of the blocks."""
         found: Dict[str, Any] = {}

@@ -498,6 +498,10 @@ class ParallelMixer(Mixer):
         both = {**self._named(self.left.state_spec(), "left"), **self._named(self.right.state_spec(), "right")}
         return both or None
 
+    def store_cache(self, store: str) -> None:
+        self.left.store_cache(store)
+        self.right.store_cache(store)
+
     def step_planners(self, kernels):
         return tuple(self.left.step_planners(kernels)) + tuple(self.right.step_planners(kernels))
 

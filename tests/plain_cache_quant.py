@@ -136,3 +136,47 @@ def _weigh(p, v, seen):
     if torch.isfinite(v).all():
         return p @ v
     return torch.stack([p[r, seen[r]] @ v[seen[r]] for r in range(p.shape[0])])
+
+
+# ---- a stand-in kernel set and a whole model over such entries ----------------------------------------------------------------
+from torch_kernels import TorchKernels  # noqa: E402
+
+
+class QuantKernels(TorchKernels):
+    """The plain kernel set of the engine's host tests, with cache entries in eight bits."""
+
+    def qkv_rope_append(self, qkv, bias, cos, sin, batch, kv, q_out, num_heads, **more):
+        if kv.spec.store is None:
+            return super().qkv_rope_append(qkv, bias, cos, sin, batch, kv, q_out, num_heads, **more)
+        wide = lambda pages: torch.zeros(pages.shape, dtype=torch.float64, device=pages.device)
+        plain = dataclasses.replace(kv, spec=dataclasses.replace(kv.spec, store=None), k_pages=wide(kv.k_pages), v_pages=wide(kv.v_pages))
+        super().qkv_rope_append(qkv, bias, cos, sin, batch, plain, q_out, num_heads, **more)
+        if not kv.writes:
+            return
+        pos = batch.positions.long()
+        page, slot = kv.block_table[batch.row_segment.long(), pos // kv.page_size].long(), pos % kv.page_size
+        for rows, codes, scales in ((plain.k_pages, kv.k_pages, kv.k_scales), (plain.v_pages, kv.v_pages, kv.v_scales)):
+            c, s = quantise(rows[page, :, slot], kv.spec.store)
+            codes.view(torch.uint8)[page, :, slot] = to_pool(c, kv.spec.store).view(torch.uint8)
+            scales[page, :, slot] = s
+
+    def paged_attention(self, q, batch, kv, out, num_heads, scale, workspace=None, **more):
+        if kv.spec.store is not None:
+            kv = dataclasses.replace(kv, spec=dataclasses.replace(kv.spec, store=None), k_pages=values(kv.k_pages, kv.k_scales),
+                                     v_pages=values(kv.v_pages, kv.v_scales))
+        super().paged_attention(q, batch, kv, out, num_heads, scale, workspace, **more)
+
+
+def logits_of(config, weights, tokens, store):
+    """Logits of one whole sequence whose layers attend to quantised keys and values."""
+    import plain_qwen2 as plain
+    x = plain.embed(weights["model.embed_tokens.weight"], tokens)
+    positions = torch.arange(len(tokens))
+    for layer in range(config["num_hidden_layers"]):
+        made = []
+        plain.block(x, weights, config, layer, positions, kv_out=made)
+        held = [values(to_pool(c, store), s).to(x.dtype) for c, s in (quantise(rows.double(), store) for rows in made[0])]
+        x = plain.block(x, weights, config, layer, positions, shared_kv=tuple(held))
+    x = plain.rms_norm(x, weights["model.norm.weight"], config["rms_norm_eps"])
+    head = weights["model.embed_tokens.weight"] if config.get("tie_word_embeddings") else weights["lm_head.weight"]
+    return plain.linear(x, head)
