@@ -11,8 +11,8 @@
 // exact in half precision, meet the weights on mma.sync m16n8k16.
 //
 // Codes are the operand with 16 rows, S^T = K Q^T and O^T = V^T P^T, so that eight query rows - the heads that share a key head,
-// times the tokens of a short portion - fill an MMA, and what a code costs on its way to half precision is paid once for up to
-// ROW_TILES eights of rows.  (Queries as the 16 rows: twice the MMAs and sums in registers for seven heads.)
+// times the tokens of a short portion - fill an MMA, and what a code costs on its way to half precision is paid once for one or two
+// eights of rows.  (Queries as the 16 rows: twice the MMAs and sums in registers for seven heads.)
 // A warp takes 32 keys at a time - a block's four in turn - and needs nothing from any other until the block's run ends.  The order of an MMA's inner index, and of its
 // rows, is free as long as all agree, so a lane's share of a tile is bytes that lie together: for the scores 16 (or 8) of a key's
 // numbers, for the sum the same of four neighbouring keys' values.  The warp copies its tiles itself, two ahead (cp.async: 512 bytes
@@ -48,10 +48,10 @@ constexpr int O_STRIDE = D + 4;
 template <int ROW_TILES>
 constexpr int warp_bytes = STAGES * STAGE_BYTES > 8 * ROW_TILES * (O_STRIDE * 4 + 8) ? STAGES * STAGE_BYTES : 8 * ROW_TILES * (O_STRIDE * 4 + 8);
 // Blocks an SM holds of the kernel for ROW_TILES eights of rows: registers allow 3 of 168 a thread, or 4 of 128, or 2 of 255.
-template <int ROW_TILES> constexpr int blocks_per_sm() { return ROW_TILES == 1 ? (D <= 64 ? 4 : 3) : ROW_TILES == 2 ? (D <= 64 ? 3 : 2) : 2; }
+template <int ROW_TILES> constexpr int blocks_per_sm() { return ROW_TILES == 1 ? (D <= 64 ? 4 : 3) : D <= 64 ? 3 : 2; }
 constexpr int MAX_SEGMENTS = 4096;
 constexpr int GROUP = 16, MOST = 32;   // pieces whose sums one block adds up: of a group, and of the last ones that are left
-constexpr int PIECE_COST = 7;          // what a piece costs beside its keys, in units
+constexpr int PIECE_COST = 12;         // what a piece costs beside its keys, in units
 constexpr float NEG_INF = -INFINITY;
 constexpr float HEADROOM = 8.f;
 
@@ -227,8 +227,9 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
     __shared__ int ticket_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-    // Few row tiles: each is cut into equal pieces of at least `share` units, a block a piece, so that none waits for a second.  `share` is
-    // such that the pieces are no more than the blocks.  Many: the line of all units, with what a piece costs beside them, is cut into equal runs.
+    // Each row tile is cut into equal pieces of at most `share` units, a block a piece, so that none waits for a second: `share` is such that the
+    // pieces are no more than the blocks.  Where that leaves the longest piece over a quarter longer, the line of all units, with what a piece
+    // costs beside them, is cut into equal runs.
     // first[s]: the pieces, or the line, before segment s.  The step's lengths are metadata that no kernel before this one writes.
     const int blocks = (int)gridDim.x;
     int units = 0, items = 0;
@@ -239,9 +240,10 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
     }
     units = __reduce_add_sync(0xffffffffu, units);
     items = __reduce_add_sync(0xffffffffu, items);
-    const bool whole = items * 8 <= blocks;
     const int total = units + items * PIECE_COST;
-    const int share = max(p.min_units, whole ? (units + blocks - items - 1) / max(1, blocks - items) : (total + blocks - 1) / blocks);
+    const int share_line = (total + blocks - 1) / blocks, share_whole = items < blocks ? (units + blocks - items - 1) / (blocks - items) : units;
+    const bool whole = items < blocks && 4 * (long long)share_whole <= 5 * (long long)max(p.min_units, share_line);
+    const int share = max(p.min_units, whole ? share_whole : share_line);
     if (warp == 0) {
         int before = 0;
         for (int base = 0; base < p.segments; base += 32) {
@@ -752,13 +754,11 @@ static int launch(Params p, int sms, long long pieces, cudaStream_t stream) {
 }
 
 constexpr int MOST_BLOCKS = 4;         // of any of the kernels, on an SM
-constexpr int MOST_TILES = D <= 64 ? 4 : 2;       // eights of rows at once: what a thread's registers hold
 
+// Sixteen rows at once where a segment has more than eight.  (Four eights, heads of 64: 37 rows of 14 heads behind 5,000 keys 20.7 us, two 17.6.)
 template <int STORE>
 static int launch_rows(const Params& p, long long rows, int sms, long long pieces, cudaStream_t stream) {
-    if (rows <= 8) return launch<STORE, 1>(p, sms, pieces, stream);
-    if (rows <= 16 || MOST_TILES == 2) return launch<STORE, 2>(p, sms, pieces, stream);
-    return launch<STORE, MOST_TILES>(p, sms, pieces, stream);
+    return rows <= 8 ? launch<STORE, 1>(p, sms, pieces, stream) : launch<STORE, 2>(p, sms, pieces, stream);
 }
 
 }  // namespace aq
@@ -767,8 +767,8 @@ static int launch_rows(const Params& p, long long rows, int sms, long long piece
 KVB_API int kvb_attention_quant_tickets() { return 7 * aq::MOST_BLOCKS; }
 KVB_API int kvb_attention_quant_scratch() {
     using namespace aq;
-    const int one = blocks_per_sm<1>() * 8, two = blocks_per_sm<2>() * 16, most = blocks_per_sm<MOST_TILES>() * 8 * MOST_TILES;
-    return 2 * (one > two ? (one > most ? one : most) : two > most ? two : most) * (D + 2);
+    const int one = blocks_per_sm<1>() * 8, two = blocks_per_sm<2>() * 16;
+    return 2 * (one > two ? one : two) * (D + 2);
 }
 
 // Segments of up to `max_q` tokens (the others' rows stay as they are).  page_size: a power of two from 4 on.  scratch and tickets:
@@ -796,7 +796,7 @@ KVB_API int kvb_attention_quant(int store, const void* q, void* out, const void*
                 block_table, table_stride, 0, segments, seg_q_start, seg_q_len, seg_kv_len, max_q, Hq, Hkv, group, reach, keep, scale, cap, sink, slopes,
                 scratch, nullptr, tickets, min_units, err};
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    // Eights of rows a block takes at once: as many as the longest segment has, as far as registers go.
+    // Eights of rows a block takes at once go by the longest segment.
     const long long most_rows = (long long)max_q * group;
     if (store == KVB_E4M3) return launch_rows<KVB_E4M3>(p, most_rows, sms, tiles * Hkv * units, stream);
     return launch_rows<KVB_INT8>(p, most_rows, sms, tiles * Hkv * units, stream);

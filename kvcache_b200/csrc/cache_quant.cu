@@ -131,7 +131,8 @@ __global__ void append_quant_any_kernel(const AppendParams p) {
 template <int LANES, int STORE, bool NORM>
 __global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendParams p, int rows) {
     constexpr int D = 8 * LANES;
-    extern __shared__ __align__(16) float angles[];          // [rows][cos, sin][rot_half]
+    // [rows][first four cosines, second four, first four sines, second four][eights of rot_half][4]: lanes read neighbouring 16 bytes.
+    extern __shared__ __align__(16) float4 angles[];
     __shared__ long long slots[APPEND_ROWS];
     // The rows' metadata and tables are older than the product before this kernel.
     const int row0 = blockIdx.x * rows, lane = threadIdx.x & 31, li = lane & (LANES - 1), d = 8 * li, half = p.rot_half;
@@ -142,10 +143,11 @@ __global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendPa
         slots[threadIdx.x] = p.write_kv ? slot_of(p, row0 + threadIdx.x, pos, true) : -1;
         angles_of(p, pos, true);
     }
-    for (int i = 4 * threadIdx.x; i < here * rot; i += 4 * blockDim.x) {
-        const int r = i / rot, at = i - r * rot;
-        const size_t angle = angles_of(p, p.positions[row0 + r], false);
-        *reinterpret_cast<float4*>(angles + i) = *reinterpret_cast<const float4*>(at < half ? p.cos_t + angle + at : p.sin_t + angle + at - half);
+    const int eights = half / 8;
+    for (int i = threadIdx.x; i < here * 4 * eights; i += blockDim.x) {
+        const int r = i / (4 * eights), c = (i - r * 4 * eights) / eights, j = i % eights;
+        const size_t angle = angles_of(p, p.positions[row0 + r], false) + 8 * j + 4 * (c & 1);
+        angles[i] = *reinterpret_cast<const float4*>((c < 2 ? p.cos_t : p.sin_t) + angle);
     }
     const bool rotated = d < rot, low = d < half;
     const int partner = (lane & ~(LANES - 1)) + (rotated ? (low ? d + half : d - half) / 8 : li);
@@ -166,10 +168,10 @@ __global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendPa
 #pragma unroll
         for (int k = 0; k < 8; ++k) { cs[k] = 1.f; sn[k] = 0.f; }
         if (rotated) {
-            const float* const at = angles + now.row * rot + (low ? d : d - half);
+            const float4* const at = angles + now.row * 4 * eights + (low ? li : li - eights);
 #pragma unroll
             for (int k = 0; k < 8; k += 4) {
-                const float4 c = *reinterpret_cast<const float4*>(at + k), s = *reinterpret_cast<const float4*>(at + half + k);
+                const float4 c = at[(k / 4) * eights], s = at[(2 + k / 4) * eights];
                 cs[k] = c.x; cs[k + 1] = c.y; cs[k + 2] = c.z; cs[k + 3] = c.w;
                 sn[k] = low ? -s.x : s.x; sn[k + 1] = low ? -s.y : s.y; sn[k + 2] = low ? -s.z : s.z; sn[k + 3] = low ? -s.w : s.w;
             }
