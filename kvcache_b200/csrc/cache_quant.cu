@@ -3,6 +3,7 @@
 //
 // The reference's cache holds half precision only (src/qwen_kernels.cu:111-126 writes it).
 #include "cache_quant.cuh"
+#include <type_traits>
 
 using namespace cq;
 
@@ -123,133 +124,157 @@ __global__ void append_quant_any_kernel(const AppendParams p) {
     if (lane == 0) (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)byte;
 }
 
-// bfloat16, heads of 8 LANES numbers, rotated halves in steps of eight: LANES lanes hold a head, eight neighbouring numbers each, and a
-// rotation partner is some lanes away.  A block takes `rows` rows, whose pages and angles it looks up once, and its groups of lanes go through
-// their heads, with three in flight.
-// Bound by the way from a row's position to its angles and by what is in flight: 2,048 rows of 36 heads of 128 (38 MB in and out) take APPEND_US
-// in blocks of four rows, 22 a block a row; a warp a head with a number a lane took 47.
+// bfloat16, heads of 16 LANES numbers, rotated halves in steps of eight: LANES lanes hold a head, eight neighbouring numbers and their eight
+// rotation partners each (of what is not rotated, eight numbers of either half).  A block takes `rows` rows, whose pages and angles it looks up
+// once, and its groups of lanes go through their heads, with three in flight.
+// Bound by instructions: 2,048 rows of 36 heads of 128 (38 MB in and out) take APPEND_US; eight numbers a lane, partners by shuffles, took 16.3, a
+// warp a head with a number a lane 47.
 template <int LANES, int STORE, bool NORM>
 __global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendParams p, int rows) {
-    constexpr int D = 8 * LANES;
+    constexpr int D = 16 * LANES;
     // [rows][first four cosines, second four, first four sines, second four][eights of rot_half][4]: lanes read neighbouring 16 bytes.
     extern __shared__ __align__(16) float4 angles[];
     __shared__ long long slots[APPEND_ROWS];
     // The rows' metadata and tables are older than the product before this kernel.
-    const int row0 = blockIdx.x * rows, lane = threadIdx.x & 31, li = lane & (LANES - 1), d = 8 * li, half = p.rot_half;
-    const uint32_t group_mask = (LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u) << (lane & ~(LANES - 1));
-    const int groups = blockDim.x / LANES, heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), rot = 2 * half, here = min(rows, p.T - row0);
+    const int row0 = blockIdx.x * rows, lane = threadIdx.x & 31, li = lane & (LANES - 1), half = p.rot_half, eights = half / 8;
+    const uint32_t group_mask = ((1u << LANES) - 1u) << (lane & ~(LANES - 1));
+    const int groups = blockDim.x / LANES, heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), here = min(rows, p.T - row0);
     if ((int)threadIdx.x < here) {
         const int pos = p.positions[row0 + threadIdx.x];
         slots[threadIdx.x] = p.write_kv ? slot_of(p, row0 + threadIdx.x, pos, true) : -1;
         angles_of(p, pos, true);
     }
-    const int eights = half / 8;
     for (int i = threadIdx.x; i < here * 4 * eights; i += blockDim.x) {
         const int r = i / (4 * eights), c = (i - r * 4 * eights) / eights, j = i % eights;
         const size_t angle = angles_of(p, p.positions[row0 + r], false) + 8 * j + 4 * (c & 1);
         angles[i] = *reinterpret_cast<const float4*>((c < 2 ? p.cos_t : p.sin_t) + angle);
     }
-    const bool rotated = d < rot, low = d < half;
-    const int partner = (lane & ~(LANES - 1)) + (rotated ? (low ? d + half : d - half) / 8 : li);
+    // This lane's first numbers, and how far the others lie behind them.
+    const bool rotated = li < eights;
+    const int d = rotated ? 8 * li : 2 * half + 8 * (li - eights), apart = rotated ? half : (D - 2 * half) / 2;
     pdl_wait();
     pdl_launch_dependents();
     __syncthreads();
-    struct Place { int row, head; };
-    auto settle = [&](Place x) { while (x.head >= heads) { x.head -= heads; ++x.row; } return x; };
-    auto load = [&](const Place& x) {
-        return x.row < here ? *reinterpret_cast<const uint4*>((const bf16*)p.qkv + (size_t)(row0 + x.row) * p.row_stride + (size_t)x.head * D + d) : make_uint4(0u, 0u, 0u, 0u);
+    struct Raw { uint4 x, y; };
+    auto load = [&](int row, int head) -> Raw {
+        if (row >= here) return {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+        const bf16* const from = (const bf16*)p.qkv + (size_t)(row0 + row) * p.row_stride + head * D + d;
+        return {*reinterpret_cast<const uint4*>(from), *reinterpret_cast<const uint4*>(from + apart)};
     };
-    Place now = settle({0, (int)threadIdx.x / LANES}), then = settle({now.row, now.head + groups}), last = settle({then.row, then.head + groups});
-    uint4 raw = load(now), next = load(then), after = load(last);
-    for (; now.row < here; now = then, then = last, last = settle({last.row, last.head + groups}), raw = next, next = after, after = load(last)) {
-        const int row = row0 + now.row, head = now.head;
-        const long long slot = slots[now.row];
-        float cs[8], sn[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) { cs[k] = 1.f; sn[k] = 0.f; }
-        if (rotated) {
-            const float4* const at = angles + now.row * 4 * eights + (low ? li : li - eights);
-#pragma unroll
-            for (int k = 0; k < 8; k += 4) {
-                const float4 c = at[(k / 4) * eights], s = at[(2 + k / 4) * eights];
-                cs[k] = c.x; cs[k + 1] = c.y; cs[k + 2] = c.z; cs[k + 3] = c.w;
-                sn[k] = low ? -s.x : s.x; sn[k + 1] = low ? -s.y : s.y; sn[k + 2] = low ? -s.z : s.z; sn[k + 3] = low ? -s.w : s.w;
-            }
-        }
-        const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
-        float b[8], w[8];
+    auto number = [](const uint4& raw, int k) {
+        const uint32_t w = k < 2 ? raw.x : k < 4 ? raw.y : k < 6 ? raw.z : raw.w;
+        return __uint_as_float(k & 1 ? w & 0xffff0000u : w << 16);
+    };
+    auto load8 = [](const float* from, float* to) {
+        const float4 x = *reinterpret_cast<const float4*>(from), y = *reinterpret_cast<const float4*>(from + 4);
+        to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w; to[4] = y.x; to[5] = y.y; to[6] = y.z; to[7] = y.w;
+    };
+    // (row, head) of this and of the next two turns; `groups` is at most a few rows' heads.
+    int row = 0, head = threadIdx.x / LANES;
+    auto settle = [&](int& r, int& h) { while (h >= heads) { h -= heads; ++r; } };
+    settle(row, head);
+    int row1 = row, head1 = head + groups;
+    settle(row1, head1);
+    int row2 = row1, head2 = head1 + groups;
+    settle(row2, head2);
+    Raw raw = load(row, head), next = load(row1, head1);
+    while (row < here) {
+        const Raw after = load(row2, head2);
         const bool is_q = head < p.Hq, is_v = head >= p.Hq + p.Hkv;
-        auto load8 = [](const float* from, float* to) {
-            const float4 x = *reinterpret_cast<const float4*>(from), y = *reinterpret_cast<const float4*>(from + 4);
-            to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w; to[4] = y.x; to[5] = y.y; to[6] = y.z; to[7] = y.w;
-        };
-        if (p.bias) load8(p.bias + (size_t)head * D + d, b);
+        float cs[8], sn[8];
+        if (rotated && !is_v) {
+            const float4* const at = angles + row * 4 * eights + li;
+            const float4 c0 = at[0], c1 = at[eights], s0 = at[2 * eights], s1 = at[3 * eights];
+            cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w; cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
+            sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w; sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
+        }
         const float* const weight = is_q ? p.q_norm : p.k_norm;
-        if (NORM && !is_v && weight) load8(weight + d, w);
-        auto number = [&](int k) { return __uint_as_float(k & 1 ? word[k >> 1] & 0xffff0000u : word[k >> 1] << 16); };
-        if (is_q) {
-            float x[8];
+        // The numbers as F, biased, normalised and turned.
+        auto make = [&](auto* x, auto* y) {
+            using F = std::remove_reference_t<decltype(*x)>;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = p.bias ? number(k) + b[k] : number(k);
+            for (int k = 0; k < 8; ++k) { x[k] = (F)number(raw.x, k); y[k] = (F)number(raw.y, k); }
+            if (p.bias) {
+                float b[8];
+                load8(p.bias + (size_t)head * D + d, b);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] += (F)b[k];
+                load8(p.bias + (size_t)head * D + d + apart, b);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] += (F)b[k];
+            }
+            if (is_v) return;
             if (NORM) {
-                float sum = 0.f;
+                F sum = 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) sum = fmaf(x[k], x[k], sum);
+                for (int k = 0; k < 8; ++k) { sum += x[k] * x[k]; sum += y[k] * y[k]; }
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(group_mask, sum, o);
-                const float inv = 1.f / sqrtf(sum / D + p.eps);
+                const F inv = (F)1 / sqrt(sum / D + (F)p.eps);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = weight ? x[k] * inv * w[k] : x[k] * inv;
+                for (int k = 0; k < 8; ++k) { x[k] *= inv; y[k] *= inv; }
+                if (weight) {
+                    float w[8];
+                    load8(weight + d, w);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] *= (F)w[k];
+                    load8(weight + d + apart, w);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k] *= (F)w[k];
+                }
             }
-            uint32_t out[4];
+            if (rotated)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const F c = (F)cs[k], s = (F)sn[k], old = x[k];
+                    x[k] = old * c - y[k] * s;
+                    y[k] = y[k] * c + old * s;
+                }
+        };
+        if (is_q) {
+            float x[8], y[8];
+            make(x, y);
+            uint32_t out[2][4];
 #pragma unroll
             for (int k = 0; k < 8; k += 2) {
-                const float a0 = __shfl_sync(group_mask, x[k], partner), a1 = __shfl_sync(group_mask, x[k + 1], partner);
-                __nv_bfloat162 y = rotated ? __floats2bfloat162_rn(fmaf(x[k], cs[k], a0 * sn[k]), fmaf(x[k + 1], cs[k + 1], a1 * sn[k + 1]))
-                                           : __floats2bfloat162_rn(x[k], x[k + 1]);
-                out[k >> 1] = *reinterpret_cast<uint32_t*>(&y);
+                __nv_bfloat162 u = __floats2bfloat162_rn(x[k], x[k + 1]), v = __floats2bfloat162_rn(y[k], y[k + 1]);
+                out[0][k >> 1] = *reinterpret_cast<uint32_t*>(&u);
+                out[1][k >> 1] = *reinterpret_cast<uint32_t*>(&v);
             }
-            *reinterpret_cast<uint4*>((bf16*)p.q_out + ((size_t)row * p.Hq + head) * D + d) = make_uint4(out[0], out[1], out[2], out[3]);
-            continue;
+            bf16* const to = (bf16*)p.q_out + ((size_t)(row0 + row) * p.Hq + head) * D + d;
+            *reinterpret_cast<uint4*>(to) = make_uint4(out[0][0], out[0][1], out[0][2], out[0][3]);
+            *reinterpret_cast<uint4*>(to + apart) = make_uint4(out[1][0], out[1][1], out[1][2], out[1][3]);
+        } else {
+            double x[8], y[8];
+            make(x, y);
+            uint32_t top = 0u;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                top = max(top, max(__float_as_uint(__double2float_ru(fabs(x[k]))), __float_as_uint(__double2float_ru(fabs(y[k])))));
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(group_mask, top, o));
+            const long long slot = slots[row];
+            if (slot >= 0) {
+                const int byte = scale_byte<STORE>(top);
+                const float down = scale_down(byte);
+                uint32_t codes[4] = {0u, 0u, 0u, 0u};
+                if (down != 0.f)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        codes[k >> 2] |= code_of<STORE>(x[k], down) << (8 * (k & 3));
+                        codes[2 + (k >> 2)] |= code_of<STORE>(y[k], down) << (8 * (k & 3));
+                    }
+                const long long at = slot + (long long)(is_v ? head - p.Hq - p.Hkv : head - p.Hq) * p.page_size;
+                uint8_t* const to = (is_v ? p.v_codes : p.k_codes) + at * D + d;
+                *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
+                *reinterpret_cast<uint2*>(to + apart) = make_uint2(codes[2], codes[3]);
+                if (li == 0) (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)byte;
+            }
         }
-        double x[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = p.bias ? (double)number(k) + (double)b[k] : (double)number(k);
-        if (!is_v) {
-            if (NORM) {
-                double sum = 0.0;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum += x[k] * x[k];
-#pragma unroll
-                for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(group_mask, sum, o);
-                const double inv = 1.0 / sqrt(sum / D + (double)p.eps);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = weight ? x[k] * inv * (double)w[k] : x[k] * inv;
-            }
-            if (rot) {
-                double y[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = __shfl_sync(group_mask, x[k], partner);
-                if (rotated)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = x[k] * (double)cs[k] + y[k] * (double)sn[k];
-            }
-        }
-        uint32_t top = 0u;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(__double2float_ru(fabs(x[k]))));
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(group_mask, top, o));
-        if (slot < 0) continue;
-        const int byte = scale_byte<STORE>(top);
-        const float down = scale_down(byte);
-        uint32_t codes[2] = {0u, 0u};
-        if (down != 0.f)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) codes[k >> 2] |= code_of<STORE>(x[k], down) << (8 * (k & 3));
-        const long long at = slot + (long long)(is_v ? head - p.Hq - p.Hkv : head - p.Hq) * p.page_size;
-        *reinterpret_cast<uint2*>((is_v ? p.v_codes : p.k_codes) + at * D + d) = make_uint2(codes[0], codes[1]);
-        if (li == 0) (is_v ? p.v_scales : p.k_scales)[at] = (uint8_t)byte;
+        row = row1; head = head1; raw = next;
+        row1 = row2; head1 = head2; next = after;
+        head2 += groups;
+        settle(row2, head2);
     }
 }
 
@@ -297,10 +322,10 @@ KVB_API int kvb_append_quant(int dtype, int store, const void* qkv, int row_stri
     const uintptr_t addresses = (uintptr_t)qkv | (uintptr_t)bias | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos_t | (uintptr_t)sin_t |
                                 (uintptr_t)q_out | (uintptr_t)k_codes | (uintptr_t)v_codes;
     if (dtype == KVB_BF16 && (addresses & 15) == 0 && row_stride % 8 == 0 && rot_half % 8 == 0) {
-        if (D == 64) return append_vec<8>(p, store, stream);
-        if (D == 128) return append_vec<16>(p, store, stream);
-        if (D == 32) return append_vec<4>(p, store, stream);
-        if (D == 256) return append_vec<32>(p, store, stream);
+        if (D == 64) return append_vec<4>(p, store, stream);
+        if (D == 128) return append_vec<8>(p, store, stream);
+        if (D == 32) return append_vec<2>(p, store, stream);
+        if (D == 256) return append_vec<16>(p, store, stream);
     }
     if (dtype == KVB_BF16) return append_any<bf16>(p, store, stream);
     if (dtype == KVB_F32) return append_any<float>(p, store, stream);
