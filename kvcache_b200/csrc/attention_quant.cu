@@ -304,7 +304,9 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         if (begin == end) continue;
         const int hk = item / c.row_tiles, row0 = (item - hk * c.row_tiles) * ROWS;
         const int rows = min(ROWS, c.q_len * p.group - row0);
-        const int pos_first = c.start + row0 / p.group, pos_last = c.start + (row0 + rows - 1) / p.group;
+        const bool one = c.q_len == 1;                        // (a division less for each of a single token's rows)
+        auto token_of = [&](int row) -> int { return one ? 0 : row / p.group; };
+        const int pos_first = c.start + token_of(row0), pos_last = c.start + token_of(row0 + rows - 1);
         const int lo_first = first_seen_key(pos_first, p.reach), lo_last = first_seen_key(pos_last, p.reach);
         const int* const table = p.block_table + (size_t)seg * p.table_stride;
 
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         uint4 raw[ROW_TILES][QN];
 #pragma unroll
         for (int j = 0; j < ROW_TILES; ++j) {
-            const int row = row0 + 8 * j + g, token = row / p.group, head = hk * p.group + row - token * p.group;
+            const int row = row0 + 8 * j + g, token = token_of(row), head = hk * p.group + row - token * p.group;
             const bf16* const from = p.q + ((size_t)(c.q_start + token) * p.Hq + head) * D + t * KU;
 #pragma unroll
             for (int k = 0; k < QN; ++k)
@@ -423,7 +425,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
             }
 #pragma unroll
             for (int e2 = 0; e2 < 2; ++e2) {
-                const int r = 8 * j + 2 * t + e2, token2 = (row0 + r) / p.group;
+                const int r = 8 * j + 2 * t + e2, token2 = token_of(row0 + r);
                 pos[j][e2] = r < rows ? c.start + token2 : 0;
                 lo[j][e2] = first_seen_key(pos[j][e2], p.reach);
                 slope[j][e2] = r < rows && p.slopes ? p.slopes[hk * p.group + row0 + r - token2 * p.group] : 0.f;
@@ -623,7 +625,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         // A block's places: of a row tile that another block has begun, and of one that it leaves to others.
         auto place_of = [&](int b) -> size_t { return (size_t)2 * b + (b > block0 ? 0 : 1); };
         auto store_row = [&](int r, int col, float4 x, float M, float L) {
-            const int row = row0 + r, token = row / p.group, head = hk * p.group + row - token * p.group;
+            const int row = row0 + r, token = token_of(row), head = hk * p.group + row - token * p.group;
             if (p.sink) L += ex2(p.sink[head] * 1.4426950408889634f - (M == NEG_INF ? 0.f : M));
             const float k = L > 0.f ? 1.f / L : L == 0.f ? 0.f : __int_as_float(0x7fffffff);
             __nv_bfloat162 a = __floats2bfloat162_rn(x.x * k, x.y * k), b = __floats2bfloat162_rn(x.z * k, x.w * k);
@@ -660,7 +662,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
             // Adds what n blocks from b0 on (every `step`th) have left, in order: (row, columns, sums, m, l) go to `put`.  A warp takes its rows by
             // itself, with the loads of CHUNK pieces in flight; little code, which only a few blocks meet, and cold.
             auto add_up = [&](int b0, int n, int step, auto put) {
-                constexpr int QUADS = D / 4, AT_ONCE = 32 / QUADS, CHUNK = 8;
+                constexpr int QUADS = D / 4, AT_ONCE = 32 / QUADS, CHUNK = 16;
 #pragma unroll 1
                 for (int r0 = warp * AT_ONCE; r0 < rows; r0 += WARPS * AT_ONCE) {
                     const int r = r0 + lane / QUADS, col = lane % QUADS * 4;

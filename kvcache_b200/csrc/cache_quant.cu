@@ -127,10 +127,10 @@ __global__ void append_quant_any_kernel(const AppendParams p) {
 // bfloat16, heads of 16 LANES numbers, rotated halves in steps of eight: LANES lanes hold a head, eight neighbouring numbers and their eight
 // rotation partners each (of what is not rotated, eight numbers of either half).  A block takes `rows` rows, whose pages and angles it looks up
 // once, and its groups of lanes go through their heads, with three in flight.
-// Bound by instructions: 2,048 rows of 36 heads of 128 (38 MB in and out) take APPEND_US; eight numbers a lane, partners by shuffles, took 16.3, a
+// Bound by instructions: 2,048 rows of 36 heads of 128 (38 MB in and out) take 10.3; eight numbers a lane, partners by shuffles, took 16.3, a
 // warp a head with a number a lane 47.
 template <int LANES, int STORE, bool NORM>
-__global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendParams p, int rows) {
+__global__ void __launch_bounds__(256, 2) append_quant_vec_kernel(const AppendParams p, int rows) {
     constexpr int D = 16 * LANES;
     // [rows][first four cosines, second four, first four sines, second four][eights of rot_half][4]: lanes read neighbouring 16 bytes.
     extern __shared__ __align__(16) float4 angles[];
@@ -280,9 +280,9 @@ __global__ void __launch_bounds__(256, 3) append_quant_vec_kernel(const AppendPa
 
 template <int LANES>
 static int append_vec(const AppendParams& p, int store, cudaStream_t stream) {
-    // A group of lanes a head; a block a row, or as many rows as leave no more blocks than the SMs hold at once (three each: with four rows a
+    // A group of lanes a head; a block a row, or as many rows as leave no more blocks than the SMs hold at once (with four rows a
     // block 2,048 rows were 512 blocks and took 24 us).
-    const int heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), wanted = (heads * LANES + 31) / 32 * 32, at_once = 3 * kvb_sm_count();
+    const int heads = p.Hq + (p.write_kv ? 2 * p.Hkv : 0), wanted = (heads * LANES + 31) / 32 * 32, at_once = 2 * kvb_sm_count();
     const int rows = (p.T + at_once - 1) / at_once < APPEND_ROWS ? (p.T + at_once - 1) / at_once : APPEND_ROWS;
     const dim3 grid((p.T + rows - 1) / rows), block(wanted < 256 ? wanted : 256);
     const size_t smem = (size_t)rows * 2 * p.rot_half * sizeof(float);

@@ -967,7 +967,7 @@ class CudaKernels(KernelSet):
         v_out = workspace.buffer(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
         stride = -(-kv.block_table.shape[1] * kv.page_size // EXPAND_BLOCK)
         table = workspace.buffer("cache.expand_table", (S, stride), torch.int32)
-        view = PagedKVView(dataclasses.replace(spec, store=None), k_out, v_out, table, EXPAND_BLOCK, False)
+        view = PagedKVView(spec.unstored, k_out, v_out, table, EXPAND_BLOCK, False)
         if n:
             self._count("cache_expand")
             _check(self._cache_quant.kvb_cache_expand(

@@ -18,7 +18,8 @@ It declares the checkpoint tensors it wants (`tensor_specs`), takes them
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+import functools
+from dataclasses import dataclass, field, replace
 from typing import Any, Dict, Mapping, Optional, Sequence, Tuple
 
 import torch
@@ -75,6 +76,11 @@ class PagedKVSpec:
     @property
     def v_head_dim(self) -> int:
         return self.head_dim if self.value_dim is None else self.value_dim
+
+    @functools.cached_property
+    def unstored(self) -> "PagedKVSpec":
+        """The same for pages in the compute type."""
+        return replace(self, store=None)
 
 
 @dataclass(frozen=True)
