@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
             // Adds what n blocks from b0 on (every `step`th) have left, in order: (row, columns, sums, m, l) go to `put`.  A warp takes its rows by
             // itself, with the loads of CHUNK pieces in flight; little code, which only a few blocks meet, and cold.
             auto add_up = [&](int b0, int n, int step, auto put) {
-                constexpr int QUADS = D / 4, AT_ONCE = 32 / QUADS, CHUNK = 16;
+                constexpr int QUADS = D / 4, AT_ONCE = 32 / QUADS, CHUNK = 8;
 #pragma unroll 1
                 for (int r0 = warp * AT_ONCE; r0 < rows; r0 += WARPS * AT_ONCE) {
                     const int r = r0 + lane / QUADS, col = lane % QUADS * 4;

@@ -423,19 +423,17 @@ template <> __device__ __forceinline__ void store8<bf16>(bf16* to, const float* 
 template <typename T, int STORE>
 __global__ void __launch_bounds__(256) expand_vec_kernel(const ExpandParams p) {
     const int i = blockIdx.x, hk = blockIdx.y, D = p.D, chunks = D >> 3;
-    const bool values = blockIdx.z == 1;
     int seg, block;
     find_block(p, i, seg, block);
     const int kv_len = p.seg_kv_len[seg], lo = first_seen_key(kv_len - p.seg_q_len[seg], p.reach), keep = p.reach > 0 ? p.keep : 0;
     const int* const table = p.block_table + (size_t)seg * p.table_stride;
-    const uint8_t* const codes = values ? p.v_codes : p.k_codes;
-    T* const out = (T*)(values ? p.v_out : p.k_out) + ((size_t)i * p.Hkv + hk) * READ_BLOCK * D;
-    constexpr int FLIGHT = 4;
+    const size_t out = ((size_t)i * p.Hkv + hk) * READ_BLOCK * D;
+    constexpr int FLIGHT = 4;                                // of keys and of values each
     bool waited = false;
     for (int c0 = threadIdx.x; c0 < READ_BLOCK * chunks; c0 += FLIGHT * 256) {
         long long at[FLIGHT];
-        uint2 code[FLIGHT];
-        float up[FLIGHT];
+        uint2 code[2][FLIGHT];
+        float up[2][FLIGHT];
 #pragma unroll
         for (int f = 0; f < FLIGHT; ++f) {
             const int c = c0 + f * 256, r = c / chunks, key = block * READ_BLOCK + r;
@@ -451,33 +449,39 @@ __global__ void __launch_bounds__(256) expand_vec_kernel(const ExpandParams p) {
             waited = true;
             pdl_wait();
             pdl_launch_dependents();
-            if (hk == 0 && !values && threadIdx.x == 0 && block < p.out_stride) p.out_table[(size_t)seg * p.out_stride + block] = i;
+            if (hk == 0 && threadIdx.x == 0 && block < p.out_stride) p.out_table[(size_t)seg * p.out_stride + block] = i;
         }
 #pragma unroll
         for (int f = 0; f < FLIGHT; ++f) {
-            code[f] = make_uint2(0u, 0u);
-            up[f] = 0.f;
+            code[0][f] = code[1][f] = make_uint2(0u, 0u);
+            up[0][f] = up[1][f] = 0.f;
             if (at[f] >= 0) {
-                code[f] = *reinterpret_cast<const uint2*>(codes + at[f] * D + ((c0 + f * 256) % chunks) * 8);
-                up[f] = read_scale(p, values, at[f]);
+                const size_t from = at[f] * D + ((c0 + f * 256) % chunks) * 8;
+                code[0][f] = *reinterpret_cast<const uint2*>(p.k_codes + from);
+                code[1][f] = *reinterpret_cast<const uint2*>(p.v_codes + from);
+                up[0][f] = read_scale(p, false, at[f]);
+                up[1][f] = read_scale(p, true, at[f]);
             }
         }
 #pragma unroll
         for (int f = 0; f < FLIGHT; ++f) {
             const int c = c0 + f * 256;
             if (c >= READ_BLOCK * chunks) break;
-            float x[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = code_value<STORE>(((k < 4 ? code[f].x : code[f].y) >> (8 * (k & 3))) & 255u) * up[f];
-            store8<T>(out + (size_t)c * 8, x);
+            for (int v = 0; v < 2; ++v) {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = code_value<STORE>(((k < 4 ? code[v][f].x : code[v][f].y) >> (8 * (k & 3))) & 255u) * up[v][f];
+                store8<T>((T*)(v ? p.v_out : p.k_out) + out + (size_t)c * 8, x);
+            }
         }
     }
 }
 
 template <typename T>
 static int expand(const ExpandParams& p, int store, int n, cudaStream_t stream) {
-    const dim3 grid(n, p.Hkv, 2);
     const bool vec = p.D % 8 == 0 && (((uintptr_t)p.k_codes | (uintptr_t)p.v_codes) & 7) == 0 && (((uintptr_t)p.k_out | (uintptr_t)p.v_out) & 15) == 0;
+    const dim3 grid(n, p.Hkv, vec ? 1 : 2);
     if (store == KVB_E4M3) kvb_launch(vec ? expand_vec_kernel<T, KVB_E4M3> : expand_any_kernel<T, KVB_E4M3>, grid, dim3(256), 0, stream, p);
     else kvb_launch(vec ? expand_vec_kernel<T, KVB_INT8> : expand_any_kernel<T, KVB_INT8>, grid, dim3(256), 0, stream, p);
     return kvb_launch_status();

@@ -48,6 +48,12 @@ class Workspace:
         self._views[key] = view
         return view
 
+    def roomy(self, name: str, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
+        """Like `buffer`, with room for the next power of two of the first dimension: what grows from step to step moves a few times only."""
+        if (name, tuple(shape), dtype) not in self._views:
+            self.buffer(name, (1 << max(int(shape[0]) - 1, 0).bit_length(), *shape[1:]), dtype)
+        return self.buffer(name, shape, dtype)
+
     def zeros(self, name: str, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
         """Like `buffer`, but zero when first made (or remade); its users leave it zero."""
         count = 1

@@ -918,6 +918,13 @@ class CudaKernels(KernelSet):
             raise KernelError("qkv_rope_append: weights for the norms of queries and keys, or for neither")
         if q_norm is not None and not norm_eps > 0.0:
             raise KernelError("qkv_rope_append: a norm's eps is above zero")
+        for name, t in (("bias", bias), ("cos", cos), ("sin", sin), ("q_norm", q_norm), ("k_norm", k_norm)):
+            if t is not None and t.dtype != torch.float32:
+                raise KernelError(f"qkv_rope_append: {name} is float32")
+        if (cos is None) != (sin is None) or (cos is not None and cos.shape != sin.shape):
+            raise KernelError("qkv_rope_append: as many sines as cosines")
+        if any(t is not None and t.numel() != D for t in (q_norm, k_norm)):
+            raise KernelError("qkv_rope_append: a norm's weights are as many as a head's numbers")
         width = (num_heads + (0 if queries_only else 2 * spec.num_kv_heads)) * D
         if qkv.shape[1] < width or q_out.dtype != qkv.dtype or q_out.numel() != T * num_heads * D or (bias is not None and bias.numel() < width):
             raise KernelError("qkv_rope_append: rows, biases or queries do not fit the heads")
@@ -963,8 +970,8 @@ class CudaKernels(KernelSet):
         n, ranges = (plan.counts["portion_blocks"], plan.arrays["portions"]) if portions else (plan.counts["blocks"], plan.arrays["ranges"])
         S, D, Hkv = batch.num_segments, spec.head_dim, spec.num_kv_heads
         name = "f32" if dtype == torch.float32 else "bf16"
-        k_out = workspace.buffer(f"cache.expand_k_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
-        v_out = workspace.buffer(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
+        k_out = workspace.roomy(f"cache.expand_k_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
+        v_out = workspace.roomy(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
         stride = -(-kv.block_table.shape[1] * kv.page_size // EXPAND_BLOCK)
         table = workspace.buffer("cache.expand_table", (S, stride), torch.int32)
         view = PagedKVView(spec.unstored, k_out, v_out, table, EXPAND_BLOCK, False)
@@ -1003,24 +1010,30 @@ class CudaKernels(KernelSet):
         T, D, Hkv, S = q.shape[0], spec.head_dim, spec.num_kv_heads, batch.num_segments
         if num_heads % Hkv or q.numel() != T * num_heads * D or out.numel() != q.numel() or out.dtype != q.dtype:
             raise KernelError("paged_attention: queries and results do not fit the heads")
+        for name, t in (("sink", sink), ("slopes", slopes)):
+            if t is not None and (t.dtype != torch.float32 or t.numel() != num_heads):
+                raise KernelError(f"paged_attention: {name} is one float32 number a query head")
+        if kv.block_table.shape[0] < S:
+            raise KernelError("paged_attention: a row of the block table for every request")
         if T == 0:
             return
         group = num_heads // Hkv
+        longest = batch.max_q_len if batch.max_q_len > 1 or T == S else T      # a batch that does not say so may still bring portions
         # Codes read in place: bfloat16, four sizes of heads, pages of at least the four keys whose scale bytes are fetched together.
-        direct = (q.dtype == torch.bfloat16 and D in (32, 64, 96, 128) and kv.page_size >= 4 and workspace is not None
+        direct = (q.dtype == torch.bfloat16 and D in (32, 64, 96, 128) and kv.page_size >= 4 and not kv.page_size & (kv.page_size - 1) and workspace is not None
                   and S <= self.QUANT_MAX_SEGMENTS and kv.k_scales.numel() < 1 << 31 and (q.data_ptr() | out.data_ptr() | kv.k_pages.data_ptr() | kv.v_pages.data_ptr()) % 16 == 0
                   and (kv.k_scales.data_ptr() | kv.v_scales.data_ptr()) % 4 == 0)
         # Read back first: portions of enough rows, and what the codes' own kernel does not take.
         expand = False
-        if not direct or (batch.max_q_len > 1 and group <= 16):
+        if not direct or (longest > 1 and group <= 16):
             plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
             paged = batch.plans.get(PagedAttentionPlanner.name)
-            singles = S if batch.max_q_len == 1 or paged is None else paged.counts["decode_items"]
+            singles = S if longest == 1 or paged is None else paged.counts["decode_items"]
             portions_only = direct or not with_singles
             blocks = 0 if plan is None else plan.counts["portion_blocks" if portions_only else "blocks"]
             expand = (blocks > 0 and paged is not None and workspace is not None and (direct or with_singles or singles == 0)
                       and 2 * q.element_size() * blocks * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES
-                      and (not direct or batch.max_q_len >= self.quant_expand_min_rows or blocks <= self.quant_expand_max_blocks * (S - singles)))
+                      and (not direct or longest >= self.quant_expand_min_rows or blocks <= self.quant_expand_max_blocks * (S - singles)))
         if expand:
             view = self.expand_cache(batch, kv, q.dtype, workspace, reach, portions_only, for_attention=True)
             portions = batch
@@ -1038,7 +1051,7 @@ class CudaKernels(KernelSet):
             _check(lib.kvb_attention_quant(
                 store, _ptr(q), _ptr(out), _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
                 _ptr(kv.block_table), kv.block_table.shape[1], S, T, _ptr(batch.seg_q_start), _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len),
-                1 if expand else batch.max_q_len, num_heads, Hkv, kv.page_size, reach, spec.keep_first, _ptr(sink), _ptr(slopes), float(score_cap or 0.0), float(scale),
+                1 if expand else longest, num_heads, Hkv, kv.page_size, reach, spec.keep_first, _ptr(sink), _ptr(slopes), float(score_cap or 0.0), float(scale),
                 _ptr(scratch), _ptr(tickets), self.sm_count, self.quant_min_units, _ptr(self.error_word), self._stream()), "paged_attention")
             return
         self._count("attention_quant_any")

@@ -102,12 +102,35 @@ def test_views_that_are_refused(changes, words):
     (dict(q_temperature=(0.1, 4)), "q_temperature"), (dict(key_dim=16), "key_dim"), (dict(value_dim=16), "value_dim"),
     (dict(queries_only=True), "queries alone"), (dict(q_norm=torch.ones(32), norm_eps=1e-6), "or for neither"),
     (dict(q_norm=torch.ones(32), k_norm=torch.ones(32)), "above zero"),
+    (dict(q_norm=torch.ones(31), k_norm=torch.ones(32), norm_eps=1e-6), "as many as"),
+    (dict(q_norm=torch.ones(32), k_norm=torch.ones(32, dtype=torch.bfloat16), norm_eps=1e-6), "k_norm is float32"),
 ])
 def test_appends_that_are_refused(more, words):
     batch, kv = _entry()
     qkv, q = torch.zeros(2, 8 * 32), torch.zeros(2, 4 * 32)
     with pytest.raises(KernelError, match=words):
         _bare().qkv_rope_append(qkv, None, None, None, batch, kv, q, 4, **more)
+
+
+def test_tables_that_are_refused():
+    batch, kv = _entry()
+    qkv, q = torch.zeros(2, 8 * 32), torch.zeros(2, 4 * 32)
+    table = torch.zeros(8, 16)
+    for bias, cos, sin, words in ((torch.zeros(255), None, None, "do not fit"), (torch.zeros(256, dtype=torch.float64), None, None, "bias is float32"),
+                                  (None, table, None, "sines"), (None, table, torch.zeros(8, 8), "sines")):
+        with pytest.raises(KernelError, match=words):
+            _bare().qkv_rope_append(qkv, bias, cos, sin, batch, kv, q, 4)
+
+
+@pytest.mark.parametrize("more, words", [
+    (dict(sink=torch.zeros(3)), "sink is one"), (dict(sink=torch.zeros(4, dtype=torch.float64)), "sink is one"), (dict(slopes=torch.zeros(5)), "slopes is one")])
+def test_attention_that_is_refused(more, words):
+    batch, kv = _entry()
+    q = torch.zeros(2, 4 * 32)
+    with pytest.raises(KernelError, match=words):
+        _bare().paged_attention(q, batch, kv, torch.zeros_like(q), 4, 1.0, **more)
+    with pytest.raises(KernelError, match="block table"):
+        _bare().paged_attention(q, batch, dataclasses.replace(kv, block_table=kv.block_table[:0]), torch.zeros_like(q), 4, 1.0)
 
 
 def test_sizes_that_are_refused():
@@ -120,3 +143,15 @@ def test_sizes_that_are_refused():
         _bare().norm_qkv_rope_append(torch.zeros(2, 64), torch.zeros(1, 64), None, torch.ones(64), 1e-6, None, None, batch, kv, torch.zeros(2, 64), 2)
     with pytest.raises(KernelError, match="list of blocks"):
         _bare().expand_cache(batch, kv, torch.bfloat16, None)
+
+
+def test_room_for_what_grows():
+    from kvcache_b200.engine.workspace import Workspace
+    ws = Workspace("cpu")
+    sizes, moved = (1, 2, 3, 5, 8, 9, 16, 4), []
+    for n in sizes:
+        view = ws.roomy("x", (n, 3), torch.float32)
+        assert view.shape == (n, 3)
+        moved.append(ws.moved)
+    assert moved == [0, 1, 2, 3, 3, 4, 4, 4] and ws._buffers["x"].numel() == 48
+    assert ws.roomy("x", (5, 3), torch.float32).data_ptr() == ws._buffers["x"].data_ptr()

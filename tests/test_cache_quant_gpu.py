@@ -284,6 +284,24 @@ def test_attention_without_lists_or_workspace(kernels, step):
     run_attention(kernels, None, *step[:5], "e4m3", plan=False, **step[5])
 
 
+def test_a_batch_that_does_not_say_how_long_its_portions_are(kernels, workspace):
+    """`max_q_len` left at its default: every row has its result all the same, and rows behind the last request's stay as they are."""
+    batch, kv = make_step([(40, 9), (3, 1)], 2, 64, 16, "int8")
+    batch = batch_to(dataclasses.replace(batch, max_q_len=1), DEV)
+    q = torch.randn(12, 8 * 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    out = torch.full_like(q, 7.0).to(DEV)
+    kernels.paged_attention(q.to(DEV), batch, kv_to(kv, DEV), out, 8, 0.125, workspace)
+    kernels.check_errors()
+    ref, size, most = plain.attention(q[:10], make_step([(40, 9), (3, 1)], 2, 64, 16, "int8")[0], kv, 8, 0.125)
+    check_attention(out[:10], ref, size, most, plain.values(kv.v_pages, kv.v_scales).abs().max(), 49, BF16)
+    assert (out[10:] == 7.0).all()
+
+
+@pytest.mark.parametrize("segments", [[(40, 1), (100, 1)], [(40, 30), (100, 1)]])
+def test_pages_of_an_odd_number_of_tokens(kernels, workspace, segments):
+    run_attention(kernels, workspace, segments, 8, 2, 64, 12, "e4m3")
+
+
 @pytest.mark.parametrize("store", plain.STORES)
 @pytest.mark.parametrize("step", [STEPS[1], STEPS[5], STEPS[8], STEPS[13], STEPS[17], STEPS[19]])
 def test_attention_in_float32(kernels, workspace, step, store):
