@@ -339,6 +339,8 @@ KVB_API int kvb_append_quant(int dtype, int store, const void* qkv, int row_stri
 // first `keep`) become zeros, whatever their pages hold.
 // `for_scores`: for a kernel that multiplies weights of zero, too, by values - a token whose key or value is not finite then gets a key of NaN,
 // which no row meets that does not see the token, and a value of zeros.
+// Neither kernel lets its successor start early (no pdl_launch_dependents): attention looks pages up, and where it can fetches keys of earlier
+// steps, before it waits, since elsewhere no kernel of the step before it writes them.  Here one does.
 constexpr int READ_BLOCK = 64;
 struct ExpandParams {
     const uint8_t* k_codes;
@@ -379,7 +381,6 @@ __device__ __forceinline__ void find_block(const ExpandParams& p, int i, int& se
 template <typename T, int STORE>
 __global__ void expand_any_kernel(const ExpandParams p) {
     pdl_wait();
-    pdl_launch_dependents();
     const int i = blockIdx.x, hk = blockIdx.y, D = p.D;
     const bool values = blockIdx.z == 1;
     int seg, block;
@@ -448,7 +449,6 @@ __global__ void __launch_bounds__(256) expand_vec_kernel(const ExpandParams p) {
         if (!waited) {                                       // up to here only what the step brought along
             waited = true;
             pdl_wait();
-            pdl_launch_dependents();
             if (hk == 0 && threadIdx.x == 0 && block < p.out_stride) p.out_table[(size_t)seg * p.out_stride + block] = i;
         }
 #pragma unroll

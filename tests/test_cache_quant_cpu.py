@@ -155,3 +155,19 @@ def test_room_for_what_grows():
         moved.append(ws.moved)
     assert moved == [0, 1, 2, 3, 3, 4, 4, 4] and ws._buffers["x"].numel() == 48
     assert ws.roomy("x", (5, 3), torch.float32).data_ptr() == ws._buffers["x"].data_ptr()
+
+
+def test_the_read_back_lets_no_successor_start_early():
+    """Attention looks pages up before it waits for the kernel in front of it, and so does what fetches keys of earlier steps.  That is sound only
+    where no kernel right before it makes them: the read-back's successor may therefore start only when the read-back has ended."""
+    import os
+    import re
+    import kvcache_b200
+    with open(os.path.join(os.path.dirname(kvcache_b200.__file__), "csrc", "cache_quant.cu")) as fh:
+        text = re.sub(r"//[^\n]*", "", fh.read())
+    kernels = {m.group(1): m.end() for m in re.finditer(r"__global__[^;{]*?(\w+_kernel)\(", text)}
+    assert {"expand_any_kernel", "expand_vec_kernel"} <= set(kernels)
+    for name in ("expand_any_kernel", "expand_vec_kernel"):
+        body = text[kernels[name]:]
+        body = body[:body.index("\n}\n")]
+        assert "pdl_wait()" in body and "pdl_launch_dependents" not in body

@@ -359,6 +359,35 @@ def test_attention_reports_pages(kernels, workspace, segments, D, page):
             kernels.check_errors()
 
 
+# Attention kernels look pages up, and may fetch keys that earlier steps have written, before the kernel in front of them has ended.
+@pytest.mark.parametrize("steps, Hq, Hkv, D, page", [
+    (([(700, 1), (90, 1), (1200, 1)], [(40, 1), (2000, 1), (333, 1)]), 8, 2, 48, 16),
+    (([(700, 1), (90, 1), (1200, 1)], [(40, 1), (2000, 1), (333, 1)]), 8, 2, 64, 24),
+    (([(700, 1), (90, 1), (1200, 1)], [(40, 1), (2000, 1), (333, 1)]), 8, 2, 128, 24),
+    (([(700, 300), (900, 500)], [(100, 200), (0, 700)]), 8, 2, 64, 16),
+    (([(700, 300), (900, 500)], [(100, 200), (0, 700)]), 16, 2, 128, 16)])
+def test_steps_in_turn_read_back_what_is_theirs(kernels, workspace, steps, Hq, Hkv, D, page):
+    """Two steps of other lengths take turns, nothing between them, in one workspace: each gets the bits that it gets alone."""
+    made = []
+    for i, segments in enumerate(steps):
+        batch, kv = make_step(segments, Hkv, D, page, "e4m3", seed=20 + i, planners=planners(kernels, (0, 0)))
+        q = torch.randn(batch.num_tokens, Hq * D, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16)
+        made.append((q.to(DEV), batch_to(batch, DEV), kv_to(kv, DEV), plain.attention(q, batch, kv, Hq, D ** -0.5), kv, segments))
+    def attend(q, batch, kv):
+        out = torch.full_like(q, float("nan"))
+        kernels.paged_attention(q, batch, kv, out, Hq, D ** -0.5, workspace)
+        return out
+    got = []
+    for _ in range(12):
+        for q, batch, kv, *_ in made:
+            got.append(attend(q, batch, kv))
+    kernels.check_errors()
+    for i, out in enumerate(got):
+        assert torch.equal(out, got[i % 2])
+    for out, (_, _, _, (ref, size, most), kv, segments) in zip(got, made):
+        check_attention(out, ref, size, most, plain.values(kv.v_pages, kv.v_scales).abs().max(), max(s + c for s, c in segments), BF16)
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("store", plain.STORES)
 def test_a_prompt_in_portions_then_tokens(kernels, workspace, store):
