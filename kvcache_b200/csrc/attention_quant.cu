@@ -42,12 +42,13 @@ constexpr int UNIT = 32;                // keys a warp takes at a time
 constexpr int KU = D % 64 == 0 ? 16 : 8, KN = D / (4 * KU);                       // bytes a read, reads of a key row by one of the four lanes that share it
 constexpr int VU = D % 128 == 0 ? 16 : D % 64 == 0 ? 8 : 4, VN = D / (8 * VU);    // ... of a value row by one of eight
 constexpr int K_BYTES = UNIT * D, STAGE_BYTES = 2 * K_BYTES + 64;                 // keys, values, and both scale bytes of a tile
-constexpr int STAGES = D <= 64 ? 3 : 2;
+constexpr int STAGES = 2;               // tiles on their way to a warp (three, heads of 64: 14 of them, 64 requests of 8,192 keys at most 30.6 us, two 28.1)
 constexpr int O_STRIDE = D + 4;
 // A warp's shared memory: its tiles, and over them its sums when a piece ends.
 template <int ROW_TILES>
 constexpr int warp_bytes = STAGES * STAGE_BYTES > 8 * ROW_TILES * (O_STRIDE * 4 + 8) ? STAGES * STAGE_BYTES : 8 * ROW_TILES * (O_STRIDE * 4 + 8);
-// Blocks an SM holds of the kernel for ROW_TILES eights of rows: registers allow 3 of 168 a thread, or 4 of 128, or 2 of 255.
+// Blocks an SM holds of the kernel for ROW_TILES eights of rows: registers allow 3 of 168 a thread, or 4 of 128, or 2 of 255
+// (five of 96, heads of 64, spill: 28.1 to 32.7 us in the case above).
 template <int ROW_TILES> constexpr int blocks_per_sm() { return ROW_TILES == 1 ? (D <= 64 ? 4 : 3) : D <= 64 ? 3 : 2; }
 constexpr int MAX_SEGMENTS = 4096;
 constexpr int GROUP = 16, MOST = 32;   // pieces whose sums one block adds up: of a group, and of the last ones that are left
@@ -791,7 +792,7 @@ KVB_API int kvb_attention_quant(int store, const void* q, void* out, const void*
     if (((uintptr_t)k_scales | (uintptr_t)v_scales) & 3) return KVB_ERR_ALIGN;
     const int group = Hq / Hkv;
     // The line of units is counted in 32 bits.
-    const long long tiles = ((long long)T * group) / 8 + segments, units = (long long)table_stride * page_size / UNIT + 3 + PIECE_COST;
+    const long long rows = min((long long)T, (long long)segments * max_q) * group, tiles = rows / 8 + segments, units = (long long)table_stride * page_size / UNIT + 3 + PIECE_COST;
     if (tiles * Hkv * units > 0x3fffffffll || (long long)table_stride * page_size > 0x3fffffffll) return KVB_ERR_LIMIT;
     if ((long long)num_pages * Hkv * page_size > 0x7fffffffll) return KVB_ERR_LIMIT;      // rows of a pool, too
     Params p = {(const bf16*)q, (bf16*)out, (const uint8_t*)k_codes, (const uint8_t*)v_codes, (const uint8_t*)k_scales, (const uint8_t*)v_scales, num_pages,
