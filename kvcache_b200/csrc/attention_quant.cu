@@ -265,8 +265,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
     const int w_begin = (int)min((long long)line, whole ? (long long)blockIdx.x : (long long)blockIdx.x * share), w_end = min(line, w_begin + (whole ? 1 : share));
     int seg = 0;
     for (int hi = p.segments; hi - seg > 1;) { const int mid = (seg + hi) >> 1; if (first[mid] <= w_begin) seg = mid; else hi = mid; }
-    pdl_wait();                                              // blocks without work as well: what comes next may count on all before it
-    pdl_launch_dependents();
+    bool waited = false;                                     // the first piece's pages are looked up before the kernel in front has ended
 
     unsigned char* const mine = smem + warp * WARP_BYTES;
     const uint32_t slots = smem_addr(mine);
@@ -372,6 +371,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         Pages ahead[STAGES + 1];
 #pragma unroll
         for (int s = 0; s <= STAGES; ++s) ahead[s] = lookup(mine_first + s * WARPS);
+        if (!waited) { waited = true; pdl_wait(); pdl_launch_dependents(); }
         // This lane's numbers of query row 8 j + g: D / 4 of them, KU together.
         constexpr int QN = D / 4 / 8;                        // 16 bytes at a time
         uint4 raw[ROW_TILES][QN];
@@ -735,6 +735,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         }
         __syncthreads();                                     // the slots are the next piece's
     }
+    if (!waited) { pdl_wait(); pdl_launch_dependents(); }    // blocks without work as well: what comes next may count on all before it
 }
 
 template <int STORE, int ROW_TILES>
