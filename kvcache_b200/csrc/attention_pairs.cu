@@ -134,6 +134,7 @@ struct Params {
     const int* seg_q_len;
     const int* seg_kv_len;
     const int* block_table;    // [segments, table_stride]
+    int made_table;            // the table is the work of the kernel in front of this one
     int table_stride, page_size, page_shift;
     const int* seg_key_row;    // expanded: where key 0 of a segment would lie among the rows of keys
     int rot_steps;             // expanded: the shared part's numbers, in sixteens
@@ -331,8 +332,9 @@ attention_pairs_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 }
                 return page;
             };
+            // Everything up to here, and the table where no kernel of the step makes it, is metadata that the host wrote at the step's start.
+            if (!waited && p.made_table) { waited = true; pdl_wait(); pdl_launch_dependents(); }
             int page_next = lookup(0);
-            // Everything up to here is the step's metadata, which the host wrote at its start.
             if (!waited) { waited = true; pdl_wait(); pdl_launch_dependents(); }
             for (int j = 0; j < n && ok; ++j, ++count) {
                 const int page = page_next;
@@ -825,7 +827,7 @@ KVB_API int kvb_attention_pairs(const void* q, void* out, const void* k_pages, c
                              const int* block_table, int table_stride, const int* tiles, int n_tiles, float* scratch,
                              int* tickets, int blocks, const int* seg_q_start, const int* seg_q_len, const int* seg_kv_len, int T,
                              int Hq, int Hkv, int page_size, int window, float scale, const float* sink, int keep_first,
-                             const float* slopes, float cap, int min_tiles, int* err, cudaStream_t stream) {
+                             const float* slopes, float cap, int min_tiles, int made_table, int* err, cudaStream_t stream) {
     using namespace apr;
     if (n_tiles <= 0) return KVB_OK;
     if (Hkv < 1 || Hq % Hkv != 0 || Hq > 65535) return KVB_ERR_SHAPE;
@@ -840,7 +842,7 @@ KVB_API int kvb_attention_pairs(const void* q, void* out, const void* k_pages, c
     rc = make_bf16_map(&mv, v_pages, pool_rows, D, D, page_size);
     if (rc != KVB_OK) return rc;
     Params p = {};
-    p.out = (bf16*)out; p.block_table = block_table; p.tiles = tiles; p.n_tiles = n_tiles;
+    p.out = (bf16*)out; p.block_table = block_table; p.made_table = made_table; p.tiles = tiles; p.n_tiles = n_tiles;
     p.seg_q_start = seg_q_start; p.seg_q_len = seg_q_len; p.seg_kv_len = seg_kv_len;
     p.tickets = tickets;
     p.table_stride = table_stride; p.Hq = Hq; p.Hkv = Hkv; p.page_size = page_size; p.q_head = D;

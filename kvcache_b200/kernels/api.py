@@ -183,7 +183,7 @@ _SIGNATURES = {
                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
         "kvb_cache_expand": [_c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_void_p, _c_int,
                              _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
-                             _c_void_p, _c_void_p],
+                             _c_int, _c_void_p, _c_void_p],
         "kvb_attention_quant_any": [_c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p,
                                     _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_float,
                                     _c_float, _c_void_p, _c_void_p],
@@ -280,7 +280,7 @@ _SIGNATURES = {
     "attention_pairs": {
         "kvb_attention_pairs": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p,
                                 _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
-                                _c_void_p, _c_int, _c_void_p, _c_float, _c_int, _c_void_p, _c_void_p],
+                                _c_void_p, _c_int, _c_void_p, _c_float, _c_int, _c_int, _c_void_p, _c_void_p],
         "kvb_attention_pairs_expanded": [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_void_p,
                                          _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p,
                                          _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
@@ -953,12 +953,14 @@ class CudaKernels(KernelSet):
         return None, False
 
     def expand_cache(self, batch: StepBatch, kv: PagedKVView, dtype: torch.dtype, workspace, reach: Optional[int] = None,
-                     portions: bool = False, for_attention: bool = False) -> PagedKVView:
+                     portions: bool = False, for_attention: bool = False, early: bool = False) -> PagedKVView:
         """The keys and values that a step's rows see in a cache entry in eight bits, as float32 or bfloat16 (which holds them
         exactly) in pages of 64 tokens that `paged_attention` takes: one page for every 64 keys of every request of the plan (see
         `cache_expand_planner`) - with `portions`, of every request that brings more than one token - in order.  Keys behind a request's last,
         and before its rows' window, are zeros.  `for_attention`: a token whose key or value is not finite has a key of NaN and a value
-        of zeros, so that rows which do not see it are none the worse.  The pages lie in the workspace and last until its next call."""
+        of zeros, so that rows which do not see it are none the worse.  `early`: the next launch is one that waits before it looks at the table or the
+        pages (the attention of portions where the view says `made`, not that of single tokens) and may start early.  The pages lie in the workspace
+        and last until its next call."""
         spec = kv.spec
         reach = spec.reach if reach is None else int(reach)
         store = self._quantised_entry(kv, "expand_cache")
@@ -974,13 +976,13 @@ class CudaKernels(KernelSet):
         v_out = workspace.roomy(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
         stride = -(-kv.block_table.shape[1] * kv.page_size // EXPAND_BLOCK)
         table = workspace.buffer("cache.expand_table", (S, stride), torch.int32)
-        view = PagedKVView(spec.unstored, k_out, v_out, table, EXPAND_BLOCK, False)
+        view = PagedKVView(spec.unstored, k_out, v_out, table, EXPAND_BLOCK, False, made=early)
         if n:
             self._count("cache_expand")
             _check(self._cache_quant.kvb_cache_expand(
                 _dtype_code(dtype), store, _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
                 _ptr(kv.block_table), kv.block_table.shape[1], kv.page_size, _ptr(ranges), S, n, _ptr(batch.seg_q_len),
-                _ptr(batch.seg_kv_len), reach, spec.keep_first, _ptr(k_out), _ptr(v_out), _ptr(table), stride, Hkv, D, int(for_attention), _ptr(self.error_word),
+                _ptr(batch.seg_kv_len), reach, spec.keep_first, _ptr(k_out), _ptr(v_out), _ptr(table), stride, Hkv, D, int(for_attention), int(early), _ptr(self.error_word),
                 self._stream()), "expand_cache")
         return view
 
@@ -1035,7 +1037,7 @@ class CudaKernels(KernelSet):
                       and 2 * q.element_size() * blocks * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES
                       and (not direct or longest >= self.quant_expand_min_rows or blocks <= self.quant_expand_max_blocks * (S - singles)))
         if expand:
-            view = self.expand_cache(batch, kv, q.dtype, workspace, reach, portions_only, for_attention=True)
+            view = self.expand_cache(batch, kv, q.dtype, workspace, reach, portions_only, for_attention=True, early=direct)    # no single tokens' kernel follows
             portions = batch
             if direct and singles:           # single tokens keep to their codes: the portions' kernels leave them out
                 portions = dataclasses.replace(batch, plans={**batch.plans, PagedAttentionPlanner.name: StepPlan(
@@ -1233,7 +1235,7 @@ class CudaKernels(KernelSet):
                     _ptr(q), _ptr(out), _ptr(kv.k_pages), _ptr(kv.v_pages), kv.k_pages.shape[0], _ptr(kv.block_table),
                     kv.block_table.shape[1], _ptr(lists["tc_pairs"]), pairs, _ptr(scratch), _ptr(tickets), self.sm_count,
                     _ptr(batch.seg_q_start), _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len), T, num_heads, Hkv, kv.page_size,
-                    reach, float(scale), _ptr(sink), keep, _ptr(slopes), cap, self.tc_pairs_min_tiles, _ptr(self.error_word),
+                    reach, float(scale), _ptr(sink), keep, _ptr(slopes), cap, self.tc_pairs_min_tiles, int(kv.made), _ptr(self.error_word),
                     self._stream()),
                     "attention_pairs")
             elif counts["tc_units"] and long_portion:

@@ -159,7 +159,8 @@ def test_room_for_what_grows():
 
 def test_the_read_back_lets_no_successor_start_early():
     """Attention looks pages up before it waits for the kernel in front of it, and so does what fetches keys of earlier steps.  That is sound only
-    where no kernel right before it makes them: the read-back's successor may therefore start only when the read-back has ended."""
+    where no kernel right before it makes them: the read-back's successor may therefore start only when the read-back has ended, unless the caller knows
+    that it waits first - as the attention of portions does, which is told."""
     import os
     import re
     import kvcache_b200
@@ -170,4 +171,8 @@ def test_the_read_back_lets_no_successor_start_early():
     for name in ("expand_any_kernel", "expand_vec_kernel"):
         body = text[kernels[name]:]
         body = body[:body.index("\n}\n")]
-        assert "pdl_wait()" in body and "pdl_launch_dependents" not in body
+        assert "pdl_wait()" in body and body.count("pdl_launch_dependents") == body.count("if (p.early) pdl_launch_dependents();") == 1
+    with open(os.path.join(os.path.dirname(kvcache_b200.__file__), "csrc", "attention_pairs.cu")) as fh:
+        pairs = re.sub(r"//[^\n]*", "", fh.read())
+    copies = pairs[pairs.index("const int* table = p.block_table"):]
+    assert copies.index("p.made_table) { waited = true; pdl_wait();") < copies.index("lookup(0)")
