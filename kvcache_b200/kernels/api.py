@@ -989,10 +989,11 @@ class CudaKernels(KernelSet):
     QUANT_MAX_SEGMENTS = 4096
     # Bytes of keys and values that a layer reads back for a step's portions; longer ones read the codes in place.
     CACHE_EXPAND_MAX_BYTES = 1 << 30
-    # Portions have their keys and values read back first from this many tokens on, and where they have no more than this many blocks of 64
-    # keys each on average.  Codes in place and read back, us, 28 heads of 128 (4 of keys): 16 rows behind none 10 and 7, behind 2,000 18 and 22,
-    # behind 16,000 42 and 107; 64 rows 14 and 9, 33 and 39, 119 and 138; 128 rows 24 and 11, 48 and 26, 217 and 79.
-    quant_expand_min_rows, quant_expand_max_blocks = 128, 16
+    # Portions have their keys and values read back first where the longest has this many tokens.  Codes in place and read back, us, 28 heads of
+    # 128 (4 of keys): 16 rows behind none 10 and 7, behind 2,000 18 and 24, behind 16,000 42 and 107; 64 rows 12 and 10, 32 and 40, 118 and
+    # 138; 112 rows 12 and 11, 45 and 56, 192 and 216; 128 rows 13 and 12, 48 and 27, 217 and 79; 192 rows 30 and 14, 67 and 43, 322 and 97.
+    # (Launched from Python, two launches take 10 us more of the host than one.)
+    quant_expand_min_rows = 128
     quant_min_units = 8                  # units of 32 keys a block of csrc/attention_quant.cu takes at least
 
     def _quant_library(self, head_dim: int) -> Tuple[_Library, int, int]:
@@ -1027,15 +1028,14 @@ class CudaKernels(KernelSet):
                   and (kv.k_scales.data_ptr() | kv.v_scales.data_ptr()) % 4 == 0)
         # Read back first: portions of enough rows, and what the codes' own kernel does not take.
         expand = False
-        if not direct or (longest > 1 and group <= 16):
+        if not direct or (longest >= self.quant_expand_min_rows and group <= 16):
             plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
             paged = batch.plans.get(PagedAttentionPlanner.name)
             singles = S if longest == 1 or paged is None else paged.counts["decode_items"]
             portions_only = direct or not with_singles
             blocks = 0 if plan is None else plan.counts["portion_blocks" if portions_only else "blocks"]
             expand = (blocks > 0 and paged is not None and workspace is not None and (direct or with_singles or singles == 0)
-                      and 2 * q.element_size() * blocks * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES
-                      and (not direct or longest >= self.quant_expand_min_rows or blocks <= self.quant_expand_max_blocks * (S - singles)))
+                      and 2 * q.element_size() * blocks * EXPAND_BLOCK * Hkv * D <= self.CACHE_EXPAND_MAX_BYTES)
         if expand:
             view = self.expand_cache(batch, kv, q.dtype, workspace, reach, portions_only, for_attention=True, early=direct)    # no single tokens' kernel follows
             portions = batch
