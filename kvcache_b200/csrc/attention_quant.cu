@@ -340,11 +340,22 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
 #pragma unroll
                     for (int f = 0; f < D / 32; ++f) copy_async(to + s * 16 * D + copy_place(at_lane, f), from + f * 512);
                 }
-            } else {                                         // edges, small pages, pages that are not there
+            } else if (p.page_shift >= 4) {                  // edges, pages that are not there
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const int half0 = key0 + 16 * s, row = row_of(pages.of[s], half0, 16);
+                    const uint8_t* const from = codes + (size_t)max(row, 0) * D + lane * 16;
+#pragma unroll
+                    for (int f = 0; f < D / 32; ++f) {
+                        const int key = half0 + (32 * f + lane) / (D / 16);
+                        copy_async<16>(to + s * 16 * D + copy_place(at_lane, f), from + f * 512, row >= 0 && key <= pos_last && (key >= lo_first || key < c_keep));
+                    }
+                }
+            } else {                                         // small pages
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
                     const int s = c / (D / 32), f = c - s * (D / 32), part = 32 * f + lane, in_half = part / (D / 16), key = key0 + 16 * s + in_half;
-                    const int row = row_of(p.page_shift >= 4 ? (s ? pages.of[1] : pages.of[0]) : page_of(key, 1), key, 1);
+                    const int row = row_of(page_of(key, 1), key, 1);
                     const bool seen = row >= 0 && key <= pos_last && (key >= lo_first || key < c_keep);
                     copy_async<16>(to + s * 16 * D + copy_place(at_lane, f), codes + (size_t)max(row, 0) * D + (part - in_half * (D / 16)) * 16, seen);
                 }
