@@ -85,6 +85,7 @@ _TYPE_LETTERS = {_c_int: "i", _c_float: "f", _c_void_p: "p", _c_longlong: "l"}
 
 
 _RETURN_CODES = {-1: "unsupported dtype", -2: "unsupported shape", -3: "misaligned operand", -4: "size beyond the kernel's limit"}
+_NOT_BUILT = (-3, -4)                # what a kernel for some sizes answers where another takes them all
 
 
 def _check(code: int, what: str) -> None:
@@ -851,9 +852,10 @@ class CudaKernels(KernelSet):
         T = qkv.shape[0]
         spec = kv.spec
         if spec.store is not None:
-            plain = {"norm_scope": norm_scope == "head", "norm_after_rotation": not norm_after_rotation, "value_mix": value_mix is None,
-                     "q_temperature": q_temperature is None, "key_dim": key_dim in (None, spec.head_dim), "value_dim": value_dim in (None, spec.head_dim)}
-            if not all(plain.values()):
+            if not (norm_scope == "head" and not norm_after_rotation and value_mix is None and q_temperature is None
+                    and key_dim in (None, spec.head_dim) and value_dim in (None, spec.head_dim)):
+                plain = {"norm_scope": norm_scope == "head", "norm_after_rotation": not norm_after_rotation, "value_mix": value_mix is None,
+                         "q_temperature": q_temperature is None, "key_dim": key_dim in (None, spec.head_dim), "value_dim": value_dim in (None, spec.head_dim)}
                 raise KernelError(f"qkv_rope_append: {', '.join(k for k, ok in plain.items() if not ok)} is not built for a cache in eight bits")
             self._append_quantised(qkv, bias, cos, sin, batch, kv, q_out, num_heads, q_norm, k_norm, norm_eps, queries_only)
             return
@@ -894,15 +896,16 @@ class CudaKernels(KernelSet):
     def _quantised_entry(self, kv: PagedKVView, what: str) -> int:
         """The store's code, after the checks of a view of such an entry."""
         spec, k, v, ks, vs = kv.spec, kv.k_pages, kv.v_pages, kv.k_scales, kv.v_scales
-        dtype = STORE_DTYPES.get(spec.store)
+        dtype, shape, D = STORE_DTYPES.get(spec.store), k.shape, spec.head_dim
         if dtype is None:
             raise KernelError(f"{what}: a cache is held as one of {', '.join(STORE_DTYPES)}, not '{spec.store}'")
-        shape = k.shape
-        if spec.v_head_dim != spec.head_dim:
+        if spec.v_head_dim != D:
             raise KernelError(f"{what}: a cache in eight bits has values as wide as keys")
-        if k.dtype != dtype or v.dtype != dtype or shape[1:] != (spec.num_kv_heads, kv.page_size, spec.head_dim) or v.shape != shape:
+        pages = shape[0] if len(shape) == 4 else 0
+        if k.dtype is not dtype or v.dtype is not dtype or shape != (pages, spec.num_kv_heads, kv.page_size, D) or v.shape != shape:
             raise KernelError(f"{what}: pages of a cache held as {spec.store} are {dtype} [pages, kv heads, page size, head size]")
-        if ks is None or vs is None or ks.dtype != torch.uint8 or vs.dtype != torch.uint8 or ks.shape != shape[:3] or vs.shape != shape[:3]:
+        rows = (pages, spec.num_kv_heads, kv.page_size)
+        if ks is None or vs is None or ks.dtype is not torch.uint8 or vs.dtype is not torch.uint8 or ks.shape != rows or vs.shape != rows:
             raise KernelError(f"{what}: a cache in eight bits has scale bytes, uint8 [pages, kv heads, page size]")
         return self._STORE_CODES[spec.store]
 
@@ -918,12 +921,13 @@ class CudaKernels(KernelSet):
             raise KernelError("qkv_rope_append: weights for the norms of queries and keys, or for neither")
         if q_norm is not None and not norm_eps > 0.0:
             raise KernelError("qkv_rope_append: a norm's eps is above zero")
-        for name, t in (("bias", bias), ("cos", cos), ("sin", sin), ("q_norm", q_norm), ("k_norm", k_norm)):
-            if t is not None and t.dtype != torch.float32:
+        for t in (bias, cos, sin, q_norm, k_norm):
+            if t is not None and t.dtype is not torch.float32:
+                name = next(n for n, x in (("bias", bias), ("cos", cos), ("sin", sin), ("q_norm", q_norm), ("k_norm", k_norm)) if x is t)
                 raise KernelError(f"qkv_rope_append: {name} is float32")
-        if (cos is None) != (sin is None) or (cos is not None and cos.shape != sin.shape):
+        if cos is not sin and (cos is None or sin is None or cos.shape != sin.shape):
             raise KernelError("qkv_rope_append: as many sines as cosines")
-        if any(t is not None and t.numel() != D for t in (q_norm, k_norm)):
+        if (q_norm is not None and q_norm.numel() != D) or (k_norm is not None and k_norm.numel() != D):
             raise KernelError("qkv_rope_append: a norm's weights are as many as a head's numbers")
         width = (num_heads + (0 if queries_only else 2 * spec.num_kv_heads)) * D
         if qkv.shape[1] < width or q_out.dtype != qkv.dtype or q_out.numel() != T * num_heads * D or (bias is not None and bias.numel() < width):
@@ -986,7 +990,6 @@ class CudaKernels(KernelSet):
                 self._stream()), "expand_cache")
         return view
 
-    QUANT_MAX_SEGMENTS = 4096
     # Bytes of keys and values that a layer reads back for a step's portions; longer ones read the codes in place.
     CACHE_EXPAND_MAX_BYTES = 1 << 30
     # Portions have their keys and values read back first where the longest has this many tokens.  Codes in place and read back, us, 28 heads of
@@ -1013,9 +1016,9 @@ class CudaKernels(KernelSet):
         T, D, Hkv, S = q.shape[0], spec.head_dim, spec.num_kv_heads, batch.num_segments
         if num_heads % Hkv or q.numel() != T * num_heads * D or out.numel() != q.numel() or out.dtype != q.dtype:
             raise KernelError("paged_attention: queries and results do not fit the heads")
-        for name, t in (("sink", sink), ("slopes", slopes)):
-            if t is not None and (t.dtype != torch.float32 or t.numel() != num_heads):
-                raise KernelError(f"paged_attention: {name} is one float32 number a query head")
+        for t in (sink, slopes):
+            if t is not None and (t.dtype is not torch.float32 or t.numel() != num_heads):
+                raise KernelError(f"paged_attention: {'sink' if t is sink else 'slopes'} is one float32 number a query head")
         if kv.block_table.shape[0] < S:
             raise KernelError("paged_attention: a row of the block table for every request")
         if T == 0:
@@ -1023,9 +1026,8 @@ class CudaKernels(KernelSet):
         group = num_heads // Hkv
         longest = batch.max_q_len if batch.max_q_len > 1 or T == S else T      # a batch that does not say so may still bring portions
         # Codes read in place: bfloat16, four sizes of heads, pages of at least the four keys whose scale bytes are fetched together.
-        direct = (q.dtype == torch.bfloat16 and D in (32, 64, 96, 128) and kv.page_size >= 4 and not kv.page_size & (kv.page_size - 1) and workspace is not None
-                  and S <= self.QUANT_MAX_SEGMENTS and kv.k_scales.numel() < 1 << 31 and (q.data_ptr() | out.data_ptr() | kv.k_pages.data_ptr() | kv.v_pages.data_ptr()) % 16 == 0
-                  and (kv.k_scales.data_ptr() | kv.v_scales.data_ptr()) % 4 == 0)
+        page = kv.page_size
+        direct = q.dtype is torch.bfloat16 and D in (32, 64, 96, 128) and page >= 4 and not page & (page - 1) and workspace is not None
         # Read back first: portions of enough rows, and what the codes' own kernel does not take.
         expand = False
         if not direct or (longest >= self.quant_expand_min_rows and group <= 16):
@@ -1049,13 +1051,15 @@ class CudaKernels(KernelSet):
             lib, floats, tickets_wanted = self._quant_library(D)
             scratch = workspace.buffer("attn.quant_scratch", (floats,), torch.float32)
             tickets = workspace.zeros("attn.quant_tickets", (tickets_wanted,), torch.int32)
-            self._count("attention_quant")
-            _check(lib.kvb_attention_quant(
+            code = lib.kvb_attention_quant(
                 store, _ptr(q), _ptr(out), _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],
                 _ptr(kv.block_table), kv.block_table.shape[1], S, T, _ptr(batch.seg_q_start), _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len),
-                1 if expand else longest, num_heads, Hkv, kv.page_size, reach, spec.keep_first, _ptr(sink), _ptr(slopes), float(score_cap or 0.0), float(scale),
-                _ptr(scratch), _ptr(tickets), self.sm_count, self.quant_min_units, _ptr(self.error_word), self._stream()), "paged_attention")
-            return
+                1 if expand else longest, num_heads, Hkv, page, reach, spec.keep_first, _ptr(sink), _ptr(slopes), float(score_cap or 0.0), float(scale),
+                _ptr(scratch), _ptr(tickets), self.sm_count, self.quant_min_units, _ptr(self.error_word), self._stream())
+            if code not in _NOT_BUILT:       # else nothing was launched: more requests or rows than it counts, rows off 16 bytes
+                self._count("attention_quant")
+                _check(code, "paged_attention")
+                return
         self._count("attention_quant_any")
         _check(self._cache_quant.kvb_attention_quant_any(
             _dtype_code(q.dtype), store, _ptr(q), _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.k_scales), _ptr(kv.v_scales), kv.k_pages.shape[0],

@@ -256,6 +256,7 @@ class GQAAttention(Mixer):
             raise ValueError(f"a cache is held as one of {', '.join(STORE_DTYPES)}, not '{store}'")
         missing = [name for name, there in (("values of another size than keys", self.value_store != self.key_store or self.value_dim != self.head_dim),
                                             ("keys wider than their numbers", self.key_store != self.head_dim),
+                                            ("heads of more than 1,024 numbers", self.head_dim > 1024),
                                             ("norms over whole projections", self.qk_norm_eps is not None and self.qk_norm_scope != "head"),
                                             ("norms after the rotation", self.qk_norm_eps is not None and self.qk_norm_after_rotation),
                                             ("blended values", self.value_mix is not None), ("a query temperature", self.q_temperature is not None)) if there]

@@ -88,6 +88,13 @@ def test_layers_that_are_taken():
         _mixer().store_cache("fp4")
 
 
+def test_heads_that_no_kernel_takes_in_eight_bits():
+    from kvcache_b200.parts.attention import GQAAttention
+    wide = GQAAttention(64, 4, 2, 1040, qkv_bias=False, out_bias=False, position=None, window=None, prefix="p.", dtype="bfloat16")
+    with pytest.raises(ValueError, match="1,024"):
+        wide.store_cache("int8")
+
+
 def test_a_model_with_pages_that_cannot_be_held_so(tmp_path):
     from kakipel_configs import CONFIGS
     from kvcache_b200.config import config_from_dict

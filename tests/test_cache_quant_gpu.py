@@ -359,6 +359,39 @@ def test_attention_reports_pages(kernels, workspace, segments, D, page):
             kernels.check_errors()
 
 
+def test_more_requests_than_one_launch_counts(kernels, workspace):
+    run_attention(kernels, workspace, [(i % 40, 1) for i in range(4100)], 2, 1, 32, 16, "e4m3", calls=1)
+
+
+@pytest.mark.parametrize("store", plain.STORES)
+@pytest.mark.parametrize("segments", [[(300, 1), (40, 1)], [(300, 20), (40, 1)], [(100, 200)]])
+def test_pools_that_start_at_odd_addresses(kernels, workspace, segments, store):
+    Hq, Hkv, D, page = 8, 2, 64, 16
+    batch, kv = make_step(segments, Hkv, D, page, store, planners=planners(kernels, (0, 0)))
+    def off_by_one(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)
+        out = flat[1:].view(t.shape)
+        out.view(torch.uint8).copy_(t.view(torch.uint8))
+        return out
+    pool = kv_to(kv, DEV)
+    odd = dataclasses.replace(pool, **{name: off_by_one(getattr(kv, name)) for name in ("k_pages", "v_pages", "k_scales", "v_scales")})
+    q = torch.randn(batch.num_tokens, Hq * D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    b, out = batch_to(batch, DEV), torch.empty(batch.num_tokens, Hq * D, dtype=torch.bfloat16, device=DEV)
+    kernels.paged_attention(q.to(DEV), b, odd, out, Hq, D ** -0.5, workspace)
+    ref, size, most = plain.attention(q, batch, kv, Hq, D ** -0.5)
+    check_attention(out, ref, size, most, plain.values(kv.v_pages, kv.v_scales).abs().max(), max(s + c for s, c in segments), BF16)
+    qkv, bias, _ = projections(batch.num_tokens, Hq, Hkv, D, torch.bfloat16, 3)
+    for entry in (pool, odd):                # the same codes, wherever the pool lies
+        kernels.qkv_rope_append(qkv.to(DEV), bias.to(DEV), None, None, b, entry, torch.empty_like(out), Hq)
+    for name in ("k_pages", "v_pages", "k_scales", "v_scales"):
+        assert torch.equal(getattr(pool, name).view(torch.uint8), getattr(odd, name).view(torch.uint8))
+    view = kernels.expand_cache(b, odd, torch.bfloat16, workspace)
+    got = view.k_pages.clone(), view.v_pages.clone()
+    view = kernels.expand_cache(b, pool, torch.bfloat16, workspace)
+    assert torch.equal(got[0], view.k_pages) and torch.equal(got[1], view.v_pages)
+    kernels.check_errors()
+
+
 # Attention kernels look pages up, and may fetch keys that earlier steps have written, before the kernel in front of them has ended.
 @pytest.mark.parametrize("steps, Hq, Hkv, D, page", [
     (([(700, 1), (90, 1), (1200, 1)], [(40, 1), (2000, 1), (333, 1)]), 8, 2, 48, 16),
