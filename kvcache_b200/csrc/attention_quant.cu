@@ -243,15 +243,22 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
     items = __reduce_add_sync(0xffffffffu, items);
     const int total = units + items * PIECE_COST;
     const int share_line = (total + blocks - 1) / blocks, share_whole = items < blocks ? (units + blocks - items - 1) / (blocks - items) : units;
-    const bool whole = items < blocks && 4 * (long long)share_whole <= 5 * (long long)max(p.min_units, share_line);
-    const int share = max(p.min_units, whole ? share_whole : share_line);
+    const bool whole = items < blocks && 4 * (long long)share_whole <= 5 * (long long)max(2 * p.min_units, share_line);
+    const int share = whole ? max(1, share_whole) : max(2 * p.min_units, share_line);
+    // No piece is smaller than a meeting of pieces is worth: none up to 2 min_units, a unit a warp (min_units) where that makes a dozen pieces at
+    // most, else two.  One token of 14 heads of 64, smallest piece 4 / 8 / 16 units, us: 200 keys 5.6 / 5.1 / 5.1, 500 6.1 / 6.9 / 7.2, 1,000 5.9 / 6.9 / 8.9,
+    // 2,000 6.6 / 6.9 / 9.2, 4,000 8.1 / 7.8 / 9.2; of 28 of 128 6.9 / 6.2 / 6.2, 7.1 / 8.4 / 9.1, 7.7 / 8.2 / 11.2, 9.1 / 9.1 / 11.7, 11.8 / 10.2 / 12.0.
+    auto pieces_of = [&](int n) -> int {
+        const int size = max(share, n <= 2 * p.min_units ? n : n <= 12 * p.min_units ? p.min_units : 2 * p.min_units);
+        return (n + size - 1) / size;
+    };
     if (warp == 0) {
         int before = 0;
         for (int base = 0; base < p.segments; base += 32) {
             int sum = 0, mine = 0;
             if (base + lane < p.segments) {
                 const Segment c = make_segment<ROWS>(p, base + lane);
-                mine = sum = c.row_tiles * p.Hkv * (whole ? (c.n + share - 1) / share : c.n + PIECE_COST);
+                mine = sum = c.row_tiles * p.Hkv * (whole ? pieces_of(c.n) : c.n + PIECE_COST);
             }
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += up; }
@@ -283,7 +290,7 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
         const int off = w - first[seg];
         int item, begin, end, block0, block1;                // a row tile, units of its list, and the blocks that have some of them
         if (whole) {
-            const int pieces = (c.n + share - 1) / share, size = (c.n + pieces - 1) / pieces;
+            const int pieces = pieces_of(c.n), size = (c.n + pieces - 1) / pieces;
             item = off / pieces;
             begin = min(c.n, (off - item * pieces) * size);
             end = min(c.n, begin + size);

@@ -997,7 +997,7 @@ class CudaKernels(KernelSet):
     # 138; 112 rows 12 and 11, 45 and 56, 192 and 216; 128 rows 13 and 12, 48 and 27, 217 and 79; 192 rows 30 and 14, 67 and 43, 322 and 97.
     # (Launched from Python, two launches take 10 us more of the host than one.)
     quant_expand_min_rows = 128
-    quant_min_units = 8                  # units of 32 keys a block of csrc/attention_quant.cu takes at least
+    quant_min_units = 4                  # units of 32 keys in the smallest piece of work of csrc/attention_quant.cu
 
     def _quant_library(self, head_dim: int) -> Tuple[_Library, int, int]:
         """(the kernels, floats of scratch, tickets)"""
