@@ -47,6 +47,7 @@ struct DecodeParams {
     // [Hq] or nullptr: with slopes, a score is cap tanh(scale q.k / cap) (cap 0: scale q.k) minus slopes[head] (p - j) for a key p - j back.
     const float* slopes = nullptr;
     float cap = 0.f, scale = 0.f;
+    int made = 0;                  // cluster and TMA kernels: table and pages are the work of a kernel of this step
 };
 
 constexpr int MAX_SPLITS = 32;
@@ -278,7 +279,8 @@ KVB_API int kvb_flash_decode(const void* q, void* out, const void* k_pages, cons
 //
 // Keys and values that earlier steps wrote do not depend on the kernel before this one in the stream, so the
 // step's segment data, the block table and the first tiles are fetched before the wait on that kernel; only
-// the queries, and tiles that hold this step's own keys, are read after it.
+// the queries, and tiles that hold this step's own keys, are read after it.  (Pages that a kernel of this step has read back:
+// table and keys are read after the wait too.  That the kernel in front lets nobody start early does not make them visible.)
 // ---------------------------------------------------------------------------------------------
 // Stages of keys/values in shared memory: two blocks share an SM.  (A block that takes most of an SM's shared
 // memory to request its whole split at once was measured slower: clusters of such blocks wait long for a place.)
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(128) flash_decode_cluster_kernel(const __grid_
             load_tile(ks + h * TILE_ELEMS, ks + (KW + h) * TILE_ELEMS, src, (my_begin + i * KW + h) * KT, key_lo, kv_len);
     };
     // The stages of the prologue are old if all their keys lie before this step's first position.
-    const bool early = (my_begin + min(n, STAGES - 1) * KW) * KT <= first_pos;
+    const bool early = !p.made && (my_begin + min(n, STAGES - 1) * KW) * KT <= first_pos;
     if (early) {
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) {
@@ -446,11 +448,11 @@ __global__ void __launch_bounds__(128) flash_decode_cluster_kernel(const __grid_
     TRACE(6)
 }
 
-// The splits as a cluster: nsplit 1..8, no scratch.
+// The splits as a cluster: nsplit 1..8, no scratch.  `made`: as for kvb_flash_decode_tma.
 KVB_API int kvb_flash_decode_cluster(const void* q, void* out, const void* k_pages, const void* v_pages,
                                      const int* block_table, int table_stride, const int* items, int n_items,
                                      const int* seg_q_start, const int* seg_q_len, const int* seg_kv_len, int Hq, int Hkv,
-                                     int page_size, int window, int nsplit, float scale, cudaStream_t stream) {
+                                     int page_size, int window, int nsplit, float scale, int made, cudaStream_t stream) {
     if (n_items <= 0) return KVB_OK;
     if (Hkv < 1 || Hq % Hkv != 0 || Hq / Hkv > 16) return KVB_ERR_SHAPE;
     if (page_size < 1 || (page_size & (page_size - 1)) != 0) return KVB_ERR_SHAPE;
@@ -463,7 +465,7 @@ KVB_API int kvb_flash_decode_cluster(const void* q, void* out, const void* k_pag
     p.table_stride = table_stride; p.Hq = Hq; p.Hkv = Hkv; p.page_size = page_size;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    p.window = window; p.nsplit = nsplit;
+    p.window = window; p.nsplit = nsplit; p.made = made;
     p.scale_log2 = scale * 1.4426950408889634f;
     auto kernel = flash_decode_cluster_kernel<CLUSTER_STAGES, CLUSTER_KW>;
     size_t smem = (size_t)CLUSTER_STAGES * 2 * CLUSTER_KW * TILE_ELEMS * sizeof(bf16);
@@ -656,6 +658,7 @@ __global__ void __launch_bounds__(160) flash_decode_tma_kernel(const __grid_cons
         // round are fetched before the wait.  Fused, all of them are old: nobody but this kernel writes the pool
         // meanwhile, and the new position's slot is made afresh in shared memory.
         const int first = min(n, STAGES);
+        if (p.made) pdl_wait();                              // nothing of pages that a kernel of this step makes is looked at before it has ended
         int first_pages[STAGES];
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) first_pages[i] = lookup(i);
@@ -971,13 +974,14 @@ KVB_API int kvb_flash_decode_tma_max_clusters(int nsplit) {
 // bias [(Hq + 2 Hkv) D] or null, cos_t / sin_t [table_len, rot_half] (rot_half 0: no rotation).
 // Where the grid's clusters all fit with one block on an SM, the blocks take a ring of four stages instead of three:
 // at 4,096 tokens over eight splits that is a block's whole share, all of it requested before the wait.
+// `made`: the table and the pages are the work of a kernel of this step, nothing of them is read before the wait.
 KVB_API int kvb_flash_decode_tma(const void* q, void* out, void* k_pages, void* v_pages, int num_pages,
                                  const int* block_table, int table_stride, const int* items, int n_items,
                                  const int* seg_q_start, const int* seg_q_len, const int* seg_kv_len, int Hq, int Hkv,
                                  int page_size, int window, int nsplit, float scale, const void* qkv, const float* bias,
                                  const float* cos_t, const float* sin_t, int rot_half, int table_len, int nsuper,
                                  float* scratch, int* tickets, const float* sink, int keep_first, const float* slopes, float cap,
-                                 int* err, cudaStream_t stream) {
+                                 int made, int* err, cudaStream_t stream) {
     using namespace dtma;
     if (n_items <= 0) return KVB_OK;
     // Several clusters per (item, kv head): `scratch` holds n_items * Hkv * nsuper * 16 * (D + 2) floats, `tickets`
@@ -989,6 +993,7 @@ KVB_API int kvb_flash_decode_tma(const void* q, void* out, void* k_pages, void* 
     if (nsplit < 1 || nsplit > MAX_CLUSTER || n_items > 65535 || Hkv > 65535) return KVB_ERR_LIMIT;
     if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return KVB_ERR_ALIGN;
     if (qkv && (items != nullptr || rot_half < 0 || 2 * rot_half > D || (rot_half > 0 && (!cos_t || !sin_t)))) return KVB_ERR_SHAPE;
+    if (qkv && made) return KVB_ERR_SHAPE;                                  // the fused form writes the pages that it reads
     if (qkv && window > 0 && keep_first > 0) return KVB_ERR_SHAPE;          // the fused form finds the new key's stage by tile number
     CUtensorMap mk, mv;
     const long long pool_rows = (long long)num_pages * Hkv * page_size;
@@ -1004,7 +1009,7 @@ KVB_API int kvb_flash_decode_tma(const void* q, void* out, void* k_pages, void* 
     p.table_stride = table_stride; p.Hq = Hq; p.Hkv = Hkv; p.page_size = page_size;
     p.page_shift = 0;
     while ((1 << p.page_shift) < page_size) ++p.page_shift;
-    p.window = window; p.nsplit = nsplit; p.nsuper = nsuper;
+    p.window = window; p.nsplit = nsplit; p.nsuper = nsuper; p.made = made;
     p.sink = sink; p.keep = keep_first;
     p.slopes = slopes; p.cap = cap; p.scale = scale;
     p.scale_log2 = scale * 1.4426950408889634f;

@@ -134,7 +134,7 @@ struct Params {
     const int* seg_q_len;
     const int* seg_kv_len;
     const int* block_table;    // [segments, table_stride]
-    int made_table;            // the table is the work of the kernel in front of this one
+    int made_table;            // the table and the pages are the work of a kernel of this step
     int table_stride, page_size, page_shift;
     const int* seg_key_row;    // expanded: where key 0 of a segment would lie among the rows of keys
     int rot_steps;             // expanded: the shared part's numbers, in sixteens

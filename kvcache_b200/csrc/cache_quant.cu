@@ -340,8 +340,9 @@ KVB_API int kvb_append_quant(int dtype, int store, const void* qkv, int row_stri
 // `for_scores`: for a kernel that multiplies weights of zero, too, by values - a token whose key or value is not finite then gets a key of NaN,
 // which no row meets that does not see the token, and a value of zeros.
 // Attention looks pages up, and where it can fetches keys of earlier steps, before it waits, since elsewhere no kernel of the step in front of it
-// writes them.  Here one does: the successor starts when the read-back has ended - or early, if `early` says that it waits first (509 rows of 28
-// heads of 128 behind 8,192 keys, with append and attention: 87 us, 90 otherwise).
+// writes them.  Here one does: attention over what is read back is told to wait first (PagedKVView.made), for only a wait makes these writes
+// visible, not that every block has ended.  `early`: it may then be placed early, too (509 rows of 28 heads of 128 behind 8,192 keys, with append and
+// attention: 87 us, 90 otherwise).
 constexpr int READ_BLOCK = 64;
 struct ExpandParams {
     const uint8_t* k_codes;

@@ -255,12 +255,12 @@ _SIGNATURES = {
                              _c_void_p, _c_int, _c_void_p, _c_float, _c_void_p],
         "kvb_flash_decode_cluster": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int,
                                      _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
-                                     _c_void_p],
+                                     _c_int, _c_void_p],
         "kvb_flash_decode_tma_max_clusters": [_c_int],
         "kvb_flash_decode_tma": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_int,
                                  _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
                                  _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p, _c_void_p,
-                                 _c_void_p, _c_int, _c_void_p, _c_float, _c_void_p, _c_void_p],
+                                 _c_void_p, _c_int, _c_void_p, _c_float, _c_int, _c_void_p, _c_void_p],
         "kvb_flash_prefill": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p,
                               _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_float, _c_void_p,
                               _c_int, _c_void_p, _c_float, _c_int, _c_void_p],
@@ -962,9 +962,9 @@ class CudaKernels(KernelSet):
         exactly) in pages of 64 tokens that `paged_attention` takes: one page for every 64 keys of every request of the plan (see
         `cache_expand_planner`) - with `portions`, of every request that brings more than one token - in order.  Keys behind a request's last,
         and before its rows' window, are zeros.  `for_attention`: a token whose key or value is not finite has a key of NaN and a value
-        of zeros, so that rows which do not see it are none the worse.  `early`: the next launch is one that waits before it looks at the table or the
-        pages (the attention of portions where the view says `made`, not that of single tokens) and may start early.  The pages lie in the workspace
-        and last until its next call."""
+        of zeros, so that rows which do not see it are none the worse.  The view says `made`: attention over it waits for the kernels before it
+        ahead of its first look at the table or the pages.  `early`: the next launch is such an attention and may be placed while this one
+        runs.  The pages lie in the workspace and last until its next call."""
         spec = kv.spec
         reach = spec.reach if reach is None else int(reach)
         store = self._quantised_entry(kv, "expand_cache")
@@ -980,7 +980,7 @@ class CudaKernels(KernelSet):
         v_out = workspace.roomy(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
         stride = -(-kv.block_table.shape[1] * kv.page_size // EXPAND_BLOCK)
         table = workspace.buffer("cache.expand_table", (S, stride), torch.int32)
-        view = PagedKVView(spec.unstored, k_out, v_out, table, EXPAND_BLOCK, False, made=early)
+        view = PagedKVView(spec.unstored, k_out, v_out, table, EXPAND_BLOCK, False, made=True)
         if n:
             self._count("cache_expand")
             _check(self._cache_quant.kvb_cache_expand(
@@ -1120,7 +1120,7 @@ class CudaKernels(KernelSet):
             None, _ptr(out), _ptr(kv.k_pages), _ptr(kv.v_pages), kv.k_pages.shape[0], _ptr(kv.block_table),
             kv.block_table.shape[1], None, n, _ptr(batch.seg_q_start), _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len),
             num_heads, Hkv, kv.page_size, spec.reach, nsplit, float(scale), _ptr(qkv), _ptr(bias), _ptr(cos), _ptr(sin),
-            0 if cos is None else cos.shape[1], 0 if cos is None else cos.shape[0], 1, None, None, None, 0, None, 0.0, _ptr(self.error_word),
+            0 if cos is None else cos.shape[1], 0 if cos is None else cos.shape[0], 1, None, None, None, 0, None, 0.0, 0, _ptr(self.error_word),
             self._stream()), "flash_decode_tma (rotation and append fused)")
         return True
 
@@ -1301,7 +1301,7 @@ class CudaKernels(KernelSet):
                             _ptr(None if n == batch.num_segments else items), n,   # every segment, in order: no list
                             _ptr(batch.seg_q_start), _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len), num_heads, Hkv,
                             kv.page_size, reach, nsplit, float(scale), None, None, None, None, 0, 0,
-                            nsuper, _ptr(scratch), _ptr(tickets), _ptr(sink), keep, _ptr(slopes), cap, _ptr(self.error_word),
+                            nsuper, _ptr(scratch), _ptr(tickets), _ptr(sink), keep, _ptr(slopes), cap, int(kv.made), _ptr(self.error_word),
                             self._stream()), "flash_decode_tma")
                         return
                     self._count("flash_decode_cluster")
@@ -1309,7 +1309,7 @@ class CudaKernels(KernelSet):
                         _ptr(q), _ptr(out), _ptr(kv.k_pages), _ptr(kv.v_pages), _ptr(kv.block_table),
                         kv.block_table.shape[1], _ptr(items), n, _ptr(batch.seg_q_start),
                         _ptr(batch.seg_q_len), _ptr(batch.seg_kv_len), num_heads, Hkv, kv.page_size, reach,
-                        nsplit, float(scale), self._stream()), "flash_decode_cluster")
+                        nsplit, float(scale), int(kv.made), self._stream()), "flash_decode_cluster")
                     return
                 nsplit = max(1, min(32, 2 * self.decode_ctas_wanted // (n * Hkv), tiles // self.decode_min_tiles))
                 scratch = workspace.buffer("attn.decode_scratch", (n * Hkv * nsplit * 16 * (D + 2),), torch.float32)

@@ -103,7 +103,8 @@ class PagedKVView:
     # With `spec.store`: the rows' scale bytes, uint8 [pages, num_kv_heads, page_size]; pages are then torch.float8_e4m3fn or torch.int8.
     k_scales: Optional[torch.Tensor] = None
     v_scales: Optional[torch.Tensor] = None
-    made: bool = False               # pages and table are being made by the kernel launched last, which lets its successor start early
+    # Pages and table are the work of a kernel of this step: whoever reads them waits for it first, whether or not it lets its successor start early.
+    made: bool = False
 
 
 class StepPlanner:

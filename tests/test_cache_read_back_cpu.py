@@ -1,0 +1,130 @@
+"""Attention over pages that a kernel of the same step has read back, without a GPU: what the launchers are told, and the kernels' source."""
+import os
+import re
+from collections import Counter
+
+import pytest
+import torch
+
+import kvcache_b200
+import plain_cache_quant as plain
+from kvcache_b200.engine.workspace import Workspace
+from kvcache_b200.kernels import api
+from kvcache_b200.kernels.attention_plan import PagedAttentionPlanner
+from kvcache_b200.kernels.cache_plan import CacheExpandPlanner
+
+
+class Launchers:
+    """In place of a library: every launch is noted, and succeeds."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def launch(*args):
+            self.calls.append((name, args))
+            return 1 << 16 if "scratch" in name or "tickets" in name or "max_clusters" in name else 0
+        return launch
+
+    def of(self, name):
+        """The last launch's parameters by their names in the C declaration."""
+        args = next(args for n, args in reversed(self.calls) if n == name)
+        for file in sorted(os.listdir(CSRC)):
+            found = re.search(r"KVB_API int %s\(([^)]*)\)" % name, source(file)) if file.endswith(".cu") else None
+            if found:
+                names = [re.search(r"(\w+)$", part.strip()).group(1) for part in found.group(1).split(",")]
+                assert len(names) == len(args) == len(api._SIGNATURES[file[:-3]][name])
+                return dict(zip(names, args))
+        raise AssertionError(name)
+
+    def names(self):
+        return [n for n, _ in self.calls if "scratch" not in n and "tickets" not in n and "max_clusters" not in n]
+
+
+CSRC = os.path.join(os.path.dirname(kvcache_b200.__file__), "csrc")
+
+
+def source(file):
+    with open(os.path.join(CSRC, file)) as fh:
+        return re.sub(r"//[^\n]*", "", fh.read())
+
+
+@pytest.fixture()
+def kernels(monkeypatch):
+    """A kernel set whose libraries note what they are told."""
+    monkeypatch.setattr(api, "_ptr", lambda t: 0 if t is None else t.data_ptr())
+    k = api.CudaKernels.__new__(api.CudaKernels)
+    k.launches, k.launch_counts, k.launch_forms, k.libraries = 0, Counter(), Counter(), Launchers()
+    k.device, k.sm_count, k.error_word = torch.device("cpu"), 148, torch.zeros(1, dtype=torch.int32)
+    k._cache_quant = k._attn_generic = k.libraries
+    k._attn_tc = k._attn_pairs = k._flash = {d: k.libraries for d in (32, 48, 64, 96, 128)}
+    k._attn_quant = {d: (k.libraries, 1 << 16, 1 << 12) for d in (32, 64, 96, 128)}
+    k._zero_slopes, k._tma_cluster_capacity = {}, {}
+    k.tc_attention_min_rows, k.tc_history_min_rows, k.tc_history_min_units = 384, 128, 3
+    k.tc_pairs_min_units, k.tc_pairs_units_a_tile, k.tc_pairs_min_tiles = 8, {64: 2, 128: 1}, 2
+    k.tc_unit_min_tiles, k.prefill_unit_min_tiles = 16, 4
+    k.flash_attention, k.decode_merge, k.decode_cluster_max, k.decode_pow2_splits = True, "tma", 8, True
+    k.decode_ctas_wanted, k.decode_min_tiles, k.decode_superclusters, k.decode_super_min_tiles = 296, 4, 16, 8
+    k._pinned_stream, k._attention_planner, k._expand_cache_planners = 0, None, {}
+    return k
+
+
+def step(kernels, segments, Hq, Hkv, D, page, dtype=torch.bfloat16, singles=True):
+    batch, kv = plain.make_step(segments, Hkv, D, page, "e4m3", planners=(PagedAttentionPlanner(), CacheExpandPlanner(0, 0, singles)))
+    return batch, kv, torch.zeros(batch.num_tokens, Hq * D, dtype=dtype)
+
+
+@pytest.mark.parametrize("early", [False, True])
+def test_what_is_read_back_says_that_it_is_made(kernels, early):
+    batch, kv, _ = step(kernels, [(40, 3), (9, 1)], 4, 2, 64, 16)
+    view = kernels.expand_cache(batch, kv, torch.bfloat16, Workspace("cpu"), early=early)
+    assert view.made and kernels.libraries.of("kvb_cache_expand")["early"] == early
+
+
+# (segments, query heads, key heads, head size, page, with lists for single tokens, the launches that read what is read back)
+@pytest.mark.parametrize("segments, Hq, Hkv, D, page, singles, readers", [
+    ([(9000, 700)], 28, 4, 128, 2, False, {"kvb_attention_pairs": "made_table"}),
+    ([(9000, 700)], 28, 4, 64, 1, False, {"kvb_attention_pairs": "made_table"}),
+    ([(9000, 700)], 28, 4, 128, 16, False, {"kvb_attention_pairs": "made_table"}),
+    ([(900, 1), (70, 1)], 8, 2, 64, 24, True, {"kvb_flash_decode_tma": "made"}),
+    ([(900, 1), (70, 1)], 8, 2, 128, 2, True, {"kvb_flash_decode_tma": "made"}),
+    ([(900, 1), (70, 1)], 8, 2, 48, 16, True, {"kvb_flash_decode_cluster": "made"}),
+    ([(9000, 700), (70, 1)], 28, 4, 128, 2, True, {"kvb_attention_pairs": "made_table", "kvb_flash_decode_tma": "made"}),
+])
+def test_attention_over_what_is_read_back_is_told_so(kernels, segments, Hq, Hkv, D, page, singles, readers):
+    batch, kv, q = step(kernels, segments, Hq, Hkv, D, page, singles=singles)
+    kernels.paged_attention(q, batch, kv, torch.empty_like(q), Hq, 0.1, Workspace("cpu"))
+    assert kernels.libraries.names() == ["kvb_cache_expand", *readers]
+    for name, parameter in readers.items():
+        assert kernels.libraries.of(name)[parameter] == 1
+    # And of pages in the compute type, which earlier steps have written: not.
+    kernels.libraries.calls.clear()
+    wide = plain.dataclasses.replace(kv, spec=kv.spec.unstored, k_pages=kv.k_pages.to(torch.bfloat16), v_pages=kv.v_pages.to(torch.bfloat16))
+    kernels.paged_attention(q, batch, wide, torch.empty_like(q), Hq, 0.1, Workspace("cpu"))
+    for name, parameter in readers.items():
+        if name in kernels.libraries.names():
+            assert kernels.libraries.of(name)[parameter] == 0
+
+
+def body_of(text, kernel):
+    body = text[re.search(r"__global__[^;{]*?\b%s\(" % kernel, text).end():]
+    return body[:body.index("\n}\n")]
+
+
+def test_attention_waits_before_it_looks_at_made_pages():
+    """Only a wait makes another kernel's writes visible, so every kernel that `paged_attention` launches waits before its first look at a table or at
+    pages - always, or where the launch says that they are made in this step."""
+    flash, generic = source("attention_flash.cu"), source("attention_generic.cu")
+    for text, kernel in ((flash, "flash_decode_kernel"), (flash, "flash_prefill_kernel"), (generic, "paged_attention_generic_kernel"),
+                         (generic, "attention_rows_kernel")):
+        body = body_of(text, kernel)
+        looks = [m.start() for m in re.finditer(r"block_table|\btable\[|k_pages|load_tile\(", body) if m.start() > body.index("{")]
+        assert body.index("pdl_wait()") < min(looks), kernel
+    units = body_of(source("attention_tc.cu"), "attention_tc_kernel")
+    assert units.index("{ pdl_wait(); pdl_launch_dependents(); }") < units.index("p.block_table")
+    cluster = body_of(flash, "flash_decode_cluster_kernel")
+    assert "const bool early = !p.made && " in cluster
+    assert re.search(r"if \(early\) \{[^}]*load_stage\(s\)", cluster).start() < cluster.index("pdl_wait()")      # the only look ahead of the wait
+    assert cluster[cluster.index("const bool early"):cluster.index("pdl_wait()")].count("load_stage(") == 1
+    tma = body_of(flash, "flash_decode_tma_kernel")
+    assert tma.index("if (p.made) pdl_wait();") < tma.index("= lookup(") and tma.index("if (p.made) pdl_wait();") < tma.index("load_stage(i, ")
