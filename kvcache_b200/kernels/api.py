@@ -1028,9 +1028,10 @@ class CudaKernels(KernelSet):
         # Codes read in place: bfloat16, four sizes of heads, pages of at least the four keys whose scale bytes are fetched together.
         page = kv.page_size
         direct = q.dtype is torch.bfloat16 and D in (32, 64, 96, 128) and page >= 4 and not page & (page - 1) and workspace is not None
-        # Read back first: portions of enough rows, and what the codes' own kernel does not take.
+        # Read back first: portions of enough rows, and what the codes' own kernel does not take.  (Beside single tokens that keep to their codes
+        # only where kernels with lists take the portions: the others go through every row, and the single tokens' keys are not read back.)
         expand = False
-        if not direct or (longest >= self.quant_expand_min_rows and group <= 16):
+        if not direct or (longest >= self.quant_expand_min_rows and group <= 16 and self.flash_attention):
             plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
             paged = batch.plans.get(PagedAttentionPlanner.name)
             singles = S if longest == 1 or paged is None else paged.counts["decode_items"]

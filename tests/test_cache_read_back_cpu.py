@@ -128,3 +128,15 @@ def test_attention_waits_before_it_looks_at_made_pages():
     assert cluster[cluster.index("const bool early"):cluster.index("pdl_wait()")].count("load_stage(") == 1
     tma = body_of(flash, "flash_decode_tma_kernel")
     assert tma.index("if (p.made) pdl_wait();") < tma.index("= lookup(") and tma.index("if (p.made) pdl_wait();") < tma.index("load_stage(i, ")
+
+
+def test_rows_whose_keys_are_not_read_back_meet_no_kernel_that_reads_them(kernels):
+    """Without the kernels that go by lists (`flash_attention` off) attention goes through every row of the step, so portions beside single tokens keep
+    to their codes as well."""
+    batch, kv, q = step(kernels, [(900, 300), (70, 1)], 8, 2, 64, 16, singles=False)
+    for on, launches in ((True, ["kvb_cache_expand", "kvb_attention_tc", "kvb_attention_quant"]), (False, ["kvb_attention_quant"])):
+        kernels.flash_attention = on
+        kernels.libraries.calls.clear()
+        kernels.paged_attention(q, batch, kv, torch.empty_like(q), 8, 0.1, Workspace("cpu"))
+        assert kernels.libraries.names() == launches
+    assert kernels.libraries.of("kvb_attention_quant")["max_q"] == 300
