@@ -82,7 +82,7 @@ class PagedAttentionPlanner(StepPlanner):
     def plan(self, starts, counts) -> Tuple[Dict[str, np.ndarray], Dict[str, int]]:
         counts = np.asarray(counts)
         S = len(counts)
-        if int(counts.sum()) == S:                       # one token per request: every segment is an item, in order
+        if (counts == 1).all():                          # one token per request: every segment is an item, in order
             return ({"decode_items": np.arange(S, dtype=np.int32)},
                     {"decode_items": S, "prefill_units": 0, "prefill_tiles": 0, "tc_units": 0, "tc_tiles": 0, "tc_pairs": 0})
         single = counts == 1
