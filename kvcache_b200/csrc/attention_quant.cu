@@ -427,8 +427,8 @@ __global__ void __launch_bounds__(THREADS, blocks_per_sm<ROW_TILES>()) attention
             }
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = top == 0u || top >= 0x7f80u ? 0 : min(100, max(-100, (int)(top >> 7) - 127));
-            const float down = __int_as_float((127 - e) << 23), up = top >= 0x7f80u ? __int_as_float(0x7fffffff) : __int_as_float((127 + e) << 23);
+            const int e = top == 0u || top >= 0x7f80u ? 0 : max(-126, (int)(top >> 7) - 127);
+            const float down = __int_as_float(e == 127 ? 0x400000 : (127 - e) << 23), up = top >= 0x7f80u ? __int_as_float(0x7fffffff) : __int_as_float((127 + e) << 23);
 #pragma unroll
             for (int k = 0; k < QN; ++k) {
                 const uint32_t x[4] = {raw[j][k].x, raw[j][k].y, raw[j][k].z, raw[j][k].w};
