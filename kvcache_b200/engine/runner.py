@@ -374,9 +374,11 @@ class ModelRunner:
             self._graphs.pop(next(iter(self._graphs)))        # the one not used for longest
         ws = self.graph_workspace
         moved = ws.moved
-        self._forward(batch, view, layout, ws, sample, token_offset)
-        if ws.moved != moved:
-            self._graphs.clear()                              # a buffer moved: graphs that hold its old address go
+        try:
+            self._forward(batch, view, layout, ws, sample, token_offset)
+        finally:
+            if ws.moved != moved:
+                self._graphs.clear()                          # a buffer moved, and be it that the step then failed: graphs that hold its old address go
         torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
         before = self.kernels.launches

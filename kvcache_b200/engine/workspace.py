@@ -20,7 +20,8 @@ class Workspace:
         self.moved = 0        # how many times an existing buffer was replaced by a larger one
         self.frozen = False   # set while a CUDA graph is captured or replayed: growing is an error
 
-    def buffer(self, name: str, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
+    def buffer(self, name: str, shape: Tuple[int, ...], dtype: torch.dtype, room: int = 0) -> torch.Tensor:
+        """`room`: a new buffer is made for this first dimension (0: for `row_capacity` rows where they are enough)."""
         key = (name, tuple(shape), dtype)
         view = self._views.get(key)
         if view is not None:
@@ -34,25 +35,27 @@ class Workspace:
                 raise RuntimeError(f"workspace buffer '{name}' would have to grow to {count} elements "
                                    f"while its addresses are pinned by a CUDA graph")
             capacity = max(count, 1)
-            if shape and 0 < int(shape[0]) <= self.row_capacity:
-                capacity = max(capacity, count // int(shape[0]) * self.row_capacity)
-            if buf is not None and buf.dtype == dtype:
-                capacity = max(capacity, buf.numel())
+            if shape and (room or 0 < int(shape[0]) <= self.row_capacity):
+                capacity = max(capacity, count // max(int(shape[0]), 1) * (room or self.row_capacity))
             if buf is not None:
-                self.moved += 1
+                if buf.dtype == dtype:
+                    capacity = max(capacity, buf.numel())
+                self.moved += 1                          # before anything can fail: the old addresses are gone from here on
+                for old in [k for k in self._views if k[0] == name]:
+                    del self._views[old]                 # views of the buffer that is replaced
+                view = buf = None                        # its memory is given back before the larger one is asked for
+                del self._buffers[name]
             buf = torch.empty(capacity, dtype=dtype, device=self.device)
             self._buffers[name] = buf
-            for old in [k for k in self._views if k[0] == name]:
-                del self._views[old]                     # views of the buffer that was replaced
         view = buf[:count].view(shape)
         self._views[key] = view
         return view
 
-    def roomy(self, name: str, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
-        """Like `buffer`, with room for the next power of two of the first dimension: what grows from step to step moves a few times only."""
-        if (name, tuple(shape), dtype) not in self._views:
-            self.buffer(name, (1 << max(int(shape[0]) - 1, 0).bit_length(), *shape[1:]), dtype)
-        return self.buffer(name, shape, dtype)
+    def roomy(self, name: str, shape: Tuple[int, ...], dtype: torch.dtype, most: int = 1 << 62) -> torch.Tensor:
+        """Like `buffer`, with room for the next power of two of the first dimension, or for `most` of it where that is less: what grows from step to
+        step moves a few times only."""
+        n = int(shape[0])
+        return self.buffer(name, shape, dtype, room=max(n, min(1 << max(n - 1, 0).bit_length(), most)))
 
     def zeros(self, name: str, shape: Tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
         """Like `buffer`, but zero when first made (or remade); its users leave it zero."""

@@ -976,8 +976,9 @@ class CudaKernels(KernelSet):
         n, ranges = (plan.counts["portion_blocks"], plan.arrays["portions"]) if portions else (plan.counts["blocks"], plan.arrays["ranges"])
         S, D, Hkv = batch.num_segments, spec.head_dim, spec.num_kv_heads
         name = "f32" if dtype == torch.float32 else "bf16"
-        k_out = workspace.roomy(f"cache.expand_k_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
-        v_out = workspace.roomy(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype)
+        most = self.CACHE_EXPAND_MAX_BYTES // (2 * dtype.itemsize * Hkv * EXPAND_BLOCK * D)
+        k_out = workspace.roomy(f"cache.expand_k_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype, most)
+        v_out = workspace.roomy(f"cache.expand_v_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype, most)
         stride = -(-kv.block_table.shape[1] * kv.page_size // EXPAND_BLOCK)
         table = workspace.buffer("cache.expand_table", (S, stride), torch.int32)
         view = PagedKVView(spec.unstored, k_out, v_out, table, EXPAND_BLOCK, False, made=True)
@@ -990,7 +991,7 @@ class CudaKernels(KernelSet):
                 self._stream()), "expand_cache")
         return view
 
-    # Bytes of keys and values that a layer reads back for a step's portions; longer ones read the codes in place.
+    # Bytes of keys and values that a layer reads back for a step's portions, and of the buffers that a workspace keeps for them; longer ones read the codes in place.
     CACHE_EXPAND_MAX_BYTES = 1 << 30
     # Portions have their keys and values read back first where the longest has this many tokens.  Codes in place and read back, us, 28 heads of
     # 128 (4 of keys): 16 rows behind none 10 and 7, behind 2,000 18 and 24, behind 16,000 42 and 107; 64 rows 12 and 10, 32 and 40, 118 and

@@ -140,3 +140,38 @@ def test_rows_whose_keys_are_not_read_back_meet_no_kernel_that_reads_them(kernel
         kernels.paged_attention(q, batch, kv, torch.empty_like(q), 8, 0.1, Workspace("cpu"))
         assert kernels.libraries.names() == launches
     assert kernels.libraries.of("kvb_attention_quant")["max_q"] == 300
+
+
+def test_a_read_back_keeps_no_more_than_its_limit(kernels):
+    """The buffers grow by powers of two, but not past the limit that decides whether keys and values are read back."""
+    block = 2 * 2 * 2 * 64 * 64                              # bytes of keys and values, two heads of 64 in bfloat16
+    kernels.CACHE_EXPAND_MAX_BYTES = 100 * block + 17
+    for capacity in (0, 48):
+        workspace, held = Workspace("cpu", row_capacity=capacity), []
+        for keys in (64 * 3, 64 * 5, 64 * 70, 64 * 100):
+            batch, kv, q = step(kernels, [(keys - 130, 130)], 4, 2, 64, 16, singles=False)
+            kernels.libraries.calls.clear()
+            kernels.paged_attention(q, batch, kv, torch.empty_like(q), 4, 0.1, workspace)
+            assert kernels.libraries.names()[0] == "kvb_cache_expand"
+            held.append(sum(workspace._buffers[f"cache.expand_{x}_bf16"].numel() for x in "kv") * 2 // block)
+        assert held == [4, 8, 100, 100]
+    batch, kv, q = step(kernels, [(64 * 101 - 130, 130)], 4, 2, 64, 16, singles=False)
+    kernels.libraries.calls.clear()
+    kernels.paged_attention(q, batch, kv, torch.empty_like(q), 4, 0.1, workspace)
+    assert kernels.libraries.names() == ["kvb_attention_quant"]
+
+
+def test_a_buffer_that_grows_is_given_back_first(monkeypatch):
+    workspace, alive = Workspace("cpu"), []
+    workspace.buffer("x", (4,), torch.float32)
+    real = torch.empty
+
+    def empty(*args, **more):
+        alive.append("x" in workspace._buffers or any(k[0] == "x" for k in workspace._views))
+        raise MemoryError
+    monkeypatch.setattr(torch, "empty", empty)
+    with pytest.raises(MemoryError):
+        workspace.buffer("x", (5,), torch.float32)
+    assert alive == [False] and workspace.moved == 1          # whoever holds the old address is told even if there is no new one
+    monkeypatch.setattr(torch, "empty", real)
+    assert workspace.buffer("x", (3,), torch.float32).shape == (3,)
