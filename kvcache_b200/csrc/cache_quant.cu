@@ -563,8 +563,9 @@ __global__ void attention_quant_any_kernel(const AttendParams p) {
             } else {
                 at = ((long long)page * p.Hkv + hk) * p.page_size + j % p.page_size;
                 float dot = 0.f;
-                for (int d = 0; d < D; ++d) dot = fmaf(q_s[d], code_value<STORE>(p.k_codes[at * D + d]), dot);
-                s = dot * scale_up(p.k_scales[at]) * p.scale;
+                const float up = scale_up(p.k_scales[at]);   // on the codes, exact, not on the sum: that of codes may leave float32 where the key's does not
+                for (int d = 0; d < D; ++d) dot = fmaf(q_s[d], code_value<STORE>(p.k_codes[at * D + d]) * up, dot);
+                s = dot * p.scale;
                 if (p.cap > 0.f) s = p.cap * tanhf(s / p.cap);
                 if (p.slopes) s -= slope * (float)(pos - j);
             }

@@ -38,17 +38,18 @@ def test_steps_in_turn_whose_pages_are_made(kernels, workspace, steps, Hq, Hkv, 
 # ---- queries of any size ------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("store", plain.STORES)
 @pytest.mark.parametrize("power", [99, 101, 110, 120, 127, 128])
-@pytest.mark.parametrize("segments", [[(40, 1), (700, 1)], [(300, 9)]])
-def test_queries_up_to_the_largest_bfloat16(kernels, workspace, segments, power, store):  # noqa: F811
+@pytest.mark.parametrize("segments, D, dtype", [([(40, 1), (700, 1)], 64, torch.bfloat16), ([(300, 9)], 64, torch.bfloat16), ([(40, 1), (300, 9)], 20, torch.bfloat16),
+                                                ([(40, 1), (300, 1)], 64, torch.float32)])
+def test_queries_up_to_the_largest_bfloat16(kernels, workspace, segments, D, dtype, power, store):  # noqa: F811
     """Keys 2^-30 times as large as usual bring the scores back into float32, where they differ by far more than a softmax needs: every row is
     the value of its best key, and nothing else."""
-    Hq, Hkv, D = 8, 2, 64
+    Hq, Hkv = 8, 2
     batch, kv = make_step(segments, Hkv, D, 16, store, seed=12)
     kv.k_scales.sub_(30)
     g = torch.Generator().manual_seed(2)
     q = (2 * torch.rand(batch.num_tokens, Hq * D, generator=g) - 1) * 0.99
     q.view(-1, D)[:, 0] = 0.99                                 # every head's largest lies below 2^power, half of it above 2^(power - 1)
-    q = (q.double() * 2.0 ** power).float().to(torch.bfloat16)
+    q = (q.double() * 2.0 ** power).float().to(torch.bfloat16).to(dtype)
     assert torch.isfinite(q).all()
     want = torch.zeros(batch.num_tokens, Hq, D, dtype=torch.float64)
     for i, (start, count) in enumerate(segments):
