@@ -251,7 +251,7 @@ class GQAAttention(Mixer):
                            None if self.value_store == self.key_store else self.value_store, self.keep_first, self.cache_chunk,
                            self.cache_store)
 
-    def store_cache(self, store: str) -> None:
+    def check_store(self, store: str) -> None:
         if store not in STORE_DTYPES:
             raise ValueError(f"a cache is held as one of {', '.join(STORE_DTYPES)}, not '{store}'")
         missing = [name for name, there in (("values of another size than keys", self.value_store != self.key_store or self.value_dim != self.head_dim),
@@ -262,6 +262,9 @@ class GQAAttention(Mixer):
                                             ("blended values", self.value_mix is not None), ("a query temperature", self.q_temperature is not None)) if there]
         if missing:
             raise ValueError(", ".join(missing))
+
+    def store_cache(self, store: str) -> None:
+        self.check_store(store)
         self.cache_store = store
 
     def step_planners(self, kernels):

@@ -259,10 +259,14 @@ class Mixer(Part):
         """None, one `StateSpec`, or `{name: StateSpec}` for a mixer that keeps several states per request."""
         return None
 
+    def check_store(self, store: str) -> None:
+        """Raises ValueError, and changes nothing, where `store_cache(store)` would."""
+        if self.cache_spec() is not None and type(self).store_cache is Mixer.store_cache:
+            raise ValueError(f"{type(self).__name__} keeps its pages in the compute type")
+
     def store_cache(self, store: str) -> None:
         """Pages are held in eight bits from now on (before any cache is made); raises ValueError for a mixer that cannot."""
-        if self.cache_spec() is not None:
-            raise ValueError(f"{type(self).__name__} keeps its pages in the compute type")
+        self.check_store(store)
 
     def step_planners(self, kernels: Any) -> Sequence[StepPlanner]:
         """The planners whose work lists this mixer's kernels read (asked of the kernel set, which owns the tiling)."""

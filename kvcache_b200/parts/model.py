@@ -134,15 +134,17 @@ class DecoderModel:
         return entries
 
     def store_cache(self, store: str) -> None:
-        """Cached keys and values in eight bits ("e4m3", "int8"); raises if a layer's mixer keeps pages that cannot be held so."""
+        """Cached keys and values in eight bits ("e4m3", "int8"); raises, and changes no layer, if some mixer keeps pages that cannot be held so."""
         problems = []
         for i, block in enumerate(self.blocks):
             try:
-                block.mixer.store_cache(store)
+                block.mixer.check_store(store)
             except ValueError as exc:
                 problems.append(f"layer {i}: {exc}")
         if problems:
             raise ValueError(f"a cache held as {store} is not built for this model: " + "; ".join(problems))
+        for block in self.blocks:
+            block.mixer.store_cache(store)
 
     def step_planners(self, kernels: Any) -> List[Any]:
         """The planners of all mixers' kernels, each once (by name), in the order of the blocks."""

@@ -498,7 +498,12 @@ class ParallelMixer(Mixer):
         both = {**self._named(self.left.state_spec(), "left"), **self._named(self.right.state_spec(), "right")}
         return both or None
 
+    def check_store(self, store: str) -> None:
+        self.left.check_store(store)
+        self.right.check_store(store)
+
     def store_cache(self, store: str) -> None:
+        self.check_store(store)                              # of both before either changes
         self.left.store_cache(store)
         self.right.store_cache(store)
 

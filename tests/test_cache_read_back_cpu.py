@@ -175,3 +175,26 @@ def test_a_buffer_that_grows_is_given_back_first(monkeypatch):
     assert alive == [False] and workspace.moved == 1          # whoever holds the old address is told even if there is no new one
     monkeypatch.setattr(torch, "empty", real)
     assert workspace.buffer("x", (3,), torch.float32).shape == (3,)
+
+
+def test_a_model_that_refuses_leaves_every_layer_as_it_was():
+    from types import SimpleNamespace
+    from kvcache_b200.parts.attention import GQAAttention
+    from kvcache_b200.parts.model import DecoderModel
+    from kvcache_b200.parts.recurrent import GatedLinearAttention, ParallelMixer
+    make = lambda **more: GQAAttention(64, 4, 2, 32, **{**dict(qkv_bias=False, out_bias=False, position=None, window=None, prefix="p.", dtype="float32"), **more})
+    taken, refused = make(), make(q_temperature=(0.1, 8))
+    for mixers in ([taken, refused], [refused, taken]):
+        model = SimpleNamespace(blocks=[SimpleNamespace(mixer=m) for m in mixers])
+        with pytest.raises(ValueError, match=f"layer {mixers.index(refused)}: a query temperature"):
+            DecoderModel.store_cache(model, "int8")
+        assert taken.cache_store is None and taken.cache_spec().store is None and refused.cache_store is None
+    both = ParallelMixer.__new__(ParallelMixer)
+    for left, right in ((taken, refused), (refused, taken)):
+        both.left, both.right = left, right
+        with pytest.raises(ValueError, match="temperature"):
+            both.store_cache("int8")
+        assert taken.cache_store is None
+    both.right, both.left = GatedLinearAttention.__new__(GatedLinearAttention), taken
+    both.store_cache("int8")
+    assert taken.cache_store == "int8" and both.left.cache_spec().store == "int8"
