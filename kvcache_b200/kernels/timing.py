@@ -31,18 +31,19 @@ def _numel_bytes(t) -> int:
     return 0 if t is None else t.numel() * t.element_size()
 
 
-def _attention_bytes(batch, kv, num_heads: int, reach=None) -> int:
-    """Keys and values of the step's requests (every key that a row sees, once per kv head), queries in, results out."""
+def _attention_bytes(batch, kv, num_heads: int, element: int, reach=None) -> int:
+    """Keys and values of the step's requests (every key that a row sees, once per kv head; with their scale bytes where they have some), queries in and
+    results out, of `element` bytes a number."""
     spec = kv.spec
     reach = spec.reach if reach is None else reach
-    element = kv.k_pages.element_size()
+    held = spec.head_dim * kv.k_pages.element_size() + (0 if kv.k_scales is None else kv.k_scales.element_size())
     host = batch.host
     if "starts" in host and "counts" in host:
         keys = int(sum(int(s + c) - first_seen(int(s), reach) for s, c in zip(host["starts"], host["counts"])))
     else:
         keys = batch.max_kv_len * batch.num_segments
     rows = batch.num_tokens * num_heads * spec.head_dim * element
-    return 2 * keys * spec.num_kv_heads * spec.head_dim * element + 2 * rows
+    return 2 * keys * spec.num_kv_heads * held + 2 * rows
 
 
 class KernelTiming:
@@ -85,10 +86,10 @@ class KernelTiming:
             return name, 2 * _numel_bytes(args[0])
         if name == "rope_append_attention":
             qkv, batch, kv, num_heads = args[0], args[4], args[5], args[7]
-            return name, _attention_bytes(batch, kv, num_heads) + _numel_bytes(qkv)
+            return name, _attention_bytes(batch, kv, num_heads, qkv.element_size()) + _numel_bytes(qkv)
         if name == "paged_attention":
             batch, kv, num_heads = args[1], args[2], args[4]
-            return name, _attention_bytes(batch, kv, num_heads, kwargs.get("reach"))
+            return name, _attention_bytes(batch, kv, num_heads, args[0].element_size(), kwargs.get("reach"))
         if name == "sample":
             return name, _numel_bytes(args[0])
         if name == "norm_add_rmsnorm":

@@ -198,3 +198,15 @@ def test_a_model_that_refuses_leaves_every_layer_as_it_was():
     both.right, both.left = GatedLinearAttention.__new__(GatedLinearAttention), taken
     both.store_cache("int8")
     assert taken.cache_store == "int8" and both.left.cache_spec().store == "int8"
+
+
+def test_bytes_that_a_timed_attention_has_to_move():
+    """Queries and results in their own type, codes and scale bytes as they are held."""
+    from kvcache_b200.kernels.timing import KernelTiming
+    batch, kv = plain.make_step([(40, 3), (9, 1)], 2, 64, 16, "int8")
+    batch.host.update(starts=[40, 9], counts=[3, 1])
+    q = torch.zeros(4, 8 * 64, dtype=torch.bfloat16)
+    rows = 2 * q.numel() * 2
+    assert KernelTiming._describe("paged_attention", (q, batch, kv, q, 8, 1.0), {}) == ("paged_attention", rows + 2 * 53 * 2 * (64 + 1))
+    wide = plain.dataclasses.replace(kv, spec=kv.spec.unstored, k_pages=kv.k_pages.to(torch.bfloat16), v_pages=kv.v_pages.to(torch.bfloat16), k_scales=None, v_scales=None)
+    assert KernelTiming._describe("paged_attention", (q, batch, wide, q, 8, 1.0), {}) == ("paged_attention", rows + 2 * 53 * 2 * 64 * 2)
