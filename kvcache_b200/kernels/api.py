@@ -349,7 +349,6 @@ class CudaKernels(KernelSet):
             raise KernelError(f"kernels are built for sm_100a; device {self.device} is sm_{major}{minor}")
         if bf16_gemm not in ("auto", "tcgen05", "cublas", "simt"):
             raise KernelError(f"unknown bf16_gemm '{bf16_gemm}'")
-        self._device_index = torch.cuda.current_device() if self.device.index is None else self.device.index
         self.bf16_gemm = bf16_gemm
         self._elementwise = _Library("elementwise")
         self._rope = _Library("rope_append")
@@ -451,13 +450,18 @@ class CudaKernels(KernelSet):
     def _stream(self) -> int:
         if self._pinned_stream is not None:
             return self._pinned_stream
-        return torch._C._cuda_getCurrentRawStream(self._device_index)      # 0.1 us, an object for the stream 1.5 us
+        return self._current_stream()
+
+    def _current_stream(self) -> int:
+        if self.device.index is None:                        # a set made for "cuda": the device that is current at the call
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device.index)       # 0.1 us, an object for the stream 1.5 us
 
     @contextlib.contextmanager
     def on_current_stream(self):
         """Within the block every launch goes to the stream that is current now (asked for once, not per launch)."""
         saved = self._pinned_stream
-        self._pinned_stream = torch._C._cuda_getCurrentRawStream(self._device_index)
+        self._pinned_stream = self._current_stream()
         try:
             yield
         finally:

@@ -210,3 +210,20 @@ def test_bytes_that_a_timed_attention_has_to_move():
     assert KernelTiming._describe("paged_attention", (q, batch, kv, q, 8, 1.0), {}) == ("paged_attention", rows + 2 * 53 * 2 * (64 + 1))
     wide = plain.dataclasses.replace(kv, spec=kv.spec.unstored, k_pages=kv.k_pages.to(torch.bfloat16), v_pages=kv.v_pages.to(torch.bfloat16), k_scales=None, v_scales=None)
     assert KernelTiming._describe("paged_attention", (q, batch, wide, q, 8, 1.0), {}) == ("paged_attention", rows + 2 * 53 * 2 * 64 * 2)
+
+
+def test_a_set_without_a_device_number_asks_for_the_current_device_at_every_call(monkeypatch):
+    from types import SimpleNamespace
+    now = [0]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(cuda_stream=100 + (now[0] if torch.device(device).index is None else torch.device(device).index)))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index)
+    k = api.CudaKernels.__new__(api.CudaKernels)
+    k._pinned_stream = None
+    for name, streams in (("cuda", [100, 103]), ("cuda:2", [102, 102])):
+        k.device, got = torch.device(name), []
+        for now[0] in (0, 3):
+            with k.on_current_stream():
+                got.append(k._stream())
+            assert k._stream() == got[-1]
+        assert got == streams
