@@ -997,11 +997,15 @@ class CudaKernels(KernelSet):
 
     # Bytes of keys and values that a layer reads back for a step's portions, and of the buffers that a workspace keeps for them; longer ones read the codes in place.
     CACHE_EXPAND_MAX_BYTES = 1 << 30
-    # Portions have their keys and values read back first where the longest has this many tokens.  Codes in place and read back, us, 28 heads of
-    # 128 (4 of keys): 16 rows behind none 10 and 7, behind 2,000 18 and 24, behind 16,000 42 and 107; 64 rows 12 and 10, 32 and 40, 118 and
-    # 138; 112 rows 12 and 11, 45 and 56, 192 and 216; 128 rows 13 and 12, 48 and 27, 217 and 79; 192 rows 30 and 14, 67 and 43, 322 and 97.
+    # Portions have their keys and values read back first where the longest has this many tokens, by the heads' size (where the read-back goes to a
+    # tensor-memory kernel, from 128 rows on, or is ahead on the mma.sync kernel).  Codes in place and read back, us, 28 heads (4 of keys), e4m3:
+    #   heads of 128, behind 2,000 keys: 16 rows 15 and 24, 112 42 and 55, 128 46 and 27, 192 63 and 43; behind 16,000: 42 and 106, 202 and 215, 230 and 77, 338 and 96
+    #   heads of 64:                     16 rows 12 and 17, 112 28 and 33, 128 31 and 21, 192 41 and 29; behind 16,000: 27 and 57, 121 and 109, 138 and 50, 201 and 65
+    #   heads of 96:                     16 rows 15 and 21, 112 36 and 46, 128 39 and 47, 192 53 and 60; behind 16,000: 36 and 95, 159 and 187, 180 and 189, 264 and 252
+    #   heads of 32:                     16 rows 9 and 13, 112 21 and 20, 128 24 and 20, 192 31 and 27; behind 16,000: 20 and 31, 90 and 66, 102 and 68, 149 and 89
+    # Behind none: heads of 128 10 and 12 (128 rows), 22 and 14 (192); of 96 9 and 10, 20 and 12; of 64 8 and 8, 12 and 9; of 32 7 and 6, 10 and 8.
     # (Launched from Python, two launches take 10 us more of the host than one.)
-    quant_expand_min_rows = 128
+    quant_expand_min_rows = {32: 128, 64: 128, 96: 192, 128: 128}
     quant_min_units = 4                  # units of 32 keys in the smallest piece of work of csrc/attention_quant.cu
 
     def _quant_library(self, head_dim: int) -> Tuple[_Library, int, int]:
@@ -1036,7 +1040,7 @@ class CudaKernels(KernelSet):
         # Read back first: portions of enough rows, and what the codes' own kernel does not take.  (Beside single tokens that keep to their codes
         # only where kernels with lists take the portions: the others go through every row, and the single tokens' keys are not read back.)
         expand = False
-        if not direct or (longest >= self.quant_expand_min_rows and group <= 16 and self.flash_attention):
+        if not direct or (longest >= self.quant_expand_min_rows[D] and group <= 16 and self.flash_attention):
             plan, with_singles = self._expand_plan(batch, reach, spec.keep_first)
             paged = batch.plans.get(PagedAttentionPlanner.name)
             singles = S if longest == 1 or paged is None else paged.counts["decode_items"]

@@ -227,3 +227,12 @@ def test_a_set_without_a_device_number_asks_for_the_current_device_at_every_call
                 got.append(k._stream())
             assert k._stream() == got[-1]
         assert got == streams
+
+
+@pytest.mark.parametrize("D, line", [(32, 128), (64, 128), (96, 192), (128, 128)])
+def test_from_how_many_rows_on_portions_are_read_back(kernels, D, line):
+    for rows in (line - 1, line):
+        batch, kv, q = step(kernels, [(2000, rows)], 28, 4, D, 16, singles=False)
+        kernels.libraries.calls.clear()
+        kernels.paged_attention(q, batch, kv, torch.empty_like(q), 28, 0.1, Workspace("cpu"))
+        assert (kernels.libraries.names()[0] == "kvb_cache_expand") == (rows == line)
