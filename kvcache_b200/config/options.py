@@ -22,7 +22,9 @@ CACHE_DTYPES = ("auto", "e4m3", "int8")
 @dataclass
 class EngineOptions:
     dtype: str = "bfloat16"
-    cache_dtype: str = "auto"              # what cached keys and values are held as: "auto" (`dtype`), "e4m3" or "int8" (eight bits a number)
+    # What cached keys and values are held as: "auto" (`dtype`), "e4m3" or "int8" (eight bits a number).  Eight bits are read in place in bfloat16 with heads of 32,
+    # 64, 96 or 128 and pages of 4 tokens or more; in other forms decoding takes many times as long as without.
+    cache_dtype: str = "auto"
     page_size: int = 16                    # tokens in a page of the cache
     num_pages: Optional[int] = None        # pages of each cache group; None: from max_cached_tokens
     max_cached_tokens: Optional[int] = None  # pool capacity in tokens when num_pages is None

@@ -127,8 +127,9 @@ __global__ void append_quant_any_kernel(const AppendParams p) {
 // bfloat16, heads of 16 LANES numbers, rotated halves in steps of eight: LANES lanes hold a head, eight neighbouring numbers and their eight
 // rotation partners each (of what is not rotated, eight numbers of either half).  A block takes `rows` rows, whose pages and angles it looks up
 // once, and its groups of lanes go through their heads, with three in flight.
-// Bound by instructions: 2,048 rows of 36 heads of 128 (38 MB in and out) take 10.3; eight numbers a lane, partners by shuffles, took 16.3, a
-// warp a head with a number a lane 47.
+// Bound by latency at sixteen warps an SM (128 registers a thread, which float64 numbers want): schedulers issue in 44 % of the clocks, no pipe is above 25 %
+// (float64 4 %), DRAM 18 %, and what warps wait for most are the rows.  2,048 rows of 36 heads of 128 (38 MB in and out) take 10.3 us; eight numbers a lane,
+// partners by shuffles, took 16.3, a warp a head with a number a lane 47.
 template <int LANES, int STORE, bool NORM>
 __global__ void __launch_bounds__(256, 2) append_quant_vec_kernel(const AppendParams p, int rows) {
     constexpr int D = 16 * LANES;
