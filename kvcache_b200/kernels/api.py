@@ -931,6 +931,8 @@ class CudaKernels(KernelSet):
                 raise KernelError(f"qkv_rope_append: {name} is float32")
         if cos is not sin and (cos is None or sin is None or cos.shape != sin.shape):
             raise KernelError("qkv_rope_append: as many sines as cosines")
+        if kv.block_table.shape[0] < batch.num_segments:
+            raise KernelError("qkv_rope_append: a row of the block table for every request")
         if (q_norm is not None and q_norm.numel() != D) or (k_norm is not None and k_norm.numel() != D):
             raise KernelError("qkv_rope_append: a norm's weights are as many as a head's numbers")
         width = (num_heads + (0 if queries_only else 2 * spec.num_kv_heads)) * D
@@ -979,6 +981,10 @@ class CudaKernels(KernelSet):
             raise KernelError(f"expand_cache: rows are read back as float32 or bfloat16, not {dtype}")
         n, ranges = (plan.counts["portion_blocks"], plan.arrays["portions"]) if portions else (plan.counts["blocks"], plan.arrays["ranges"])
         S, D, Hkv = batch.num_segments, spec.head_dim, spec.num_kv_heads
+        if kv.block_table.shape[0] < S or ranges.numel() < 3 * (S + 1):
+            raise KernelError("expand_cache: a row of the block table, and of the list of blocks, for every request")
+        if workspace is None:
+            raise KernelError("expand_cache: the pages lie in a workspace")
         name = "f32" if dtype == torch.float32 else "bf16"
         most = self.CACHE_EXPAND_MAX_BYTES // (2 * dtype.itemsize * Hkv * EXPAND_BLOCK * D)
         k_out = workspace.roomy(f"cache.expand_k_{name}", (n, Hkv, EXPAND_BLOCK, D), dtype, most)

@@ -236,3 +236,18 @@ def test_from_how_many_rows_on_portions_are_read_back(kernels, D, line):
         kernels.libraries.calls.clear()
         kernels.paged_attention(q, batch, kv, torch.empty_like(q), 28, 0.1, Workspace("cpu"))
         assert (kernels.libraries.names()[0] == "kvb_cache_expand") == (rows == line)
+
+
+def test_calls_whose_tables_are_shorter_than_the_step_are_refused(kernels):
+    batch, kv, q = step(kernels, [(40, 3), (9, 1)], 4, 2, 64, 16)
+    short = plain.dataclasses.replace(kv, block_table=kv.block_table[:1])
+    with pytest.raises(api.KernelError, match="block table"):
+        kernels.expand_cache(batch, short, torch.bfloat16, Workspace("cpu"))
+    with pytest.raises(api.KernelError, match="block table"):
+        kernels.qkv_rope_append(torch.zeros(4, 8 * 64, dtype=torch.bfloat16), None, None, None, batch, short, q, 4)
+    other, _, _ = step(kernels, [(40, 3)], 4, 2, 64, 16)
+    with pytest.raises(api.KernelError, match="list of blocks"):
+        kernels.expand_cache(plain.dataclasses.replace(batch, plans=other.plans), kv, torch.bfloat16, Workspace("cpu"))
+    with pytest.raises(api.KernelError, match="workspace"):
+        kernels.expand_cache(batch, kv, torch.bfloat16, None)
+    assert not kernels.libraries.calls
