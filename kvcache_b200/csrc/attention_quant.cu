@@ -48,7 +48,8 @@ constexpr int O_STRIDE = D + 4;
 template <int ROW_TILES>
 constexpr int warp_bytes = STAGES * STAGE_BYTES > 8 * ROW_TILES * (O_STRIDE * 4 + 8) ? STAGES * STAGE_BYTES : 8 * ROW_TILES * (O_STRIDE * 4 + 8);
 // Blocks an SM holds of the kernel for ROW_TILES eights of rows: registers allow 3 of 168 a thread, or 4 of 128, or 2 of 255
-// (five of 96, heads of 64, spill: 28.1 to 32.7 us in the case above).
+// (five of 96, heads of 64, spill: 28.1 to 32.7 us in the case above).  Under these bounds the e4m3 instances spill 28 and 80 bytes (heads of 64, eight and sixteen
+// rows), 20 and 64 (128), 0 and 4 (96), the others none.
 template <int ROW_TILES> constexpr int blocks_per_sm() { return ROW_TILES == 1 ? (D <= 64 ? 4 : 3) : D <= 64 ? 3 : 2; }
 constexpr int MAX_SEGMENTS = 4096;
 constexpr int GROUP = 16, MOST = 32;   // pieces whose sums one block adds up: of a group, and of the last ones that are left
